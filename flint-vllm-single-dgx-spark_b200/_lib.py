@@ -92,6 +92,17 @@ SIGNATURES: dict[str, tuple] = {
     "flint_marlin_nvfp4_unpack": (I32, [P, P, P, I64, I64, I64, P, P, P, P, I32, P]),
     "flint_decode_attention": (I32, [P, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, F32, I64, I64, P, I64, I64, P,
                                      I32, P]),
+    "flint_prefill_attention_workspace_bytes": (I64, [I64, I64, I64, I64]),
+    "flint_prefill_attention": (I32, [P, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, P, I64, F32, I64, I64, I64, P, I64,
+                                      P, I32, P]),
+    "flint_shared_prefix_attention_workspace_bytes": (I64, [I64, I64, I64, I64]),
+    "flint_shared_prefix_attention": (I32, [P, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, P, I64, P, I64, F32, I64, I64,
+                                            P, I64, P, I32, P]),
+    "flint_kv_pages_workspace_bytes": (I64, [I64]),
+    "flint_kv_reserve": (I32, [P, I64, P, I64, I64, P, I64, P, P, I64, P, I32, P]),
+    "flint_kv_fork": (I32, [P, I64, I64, I64, I64, P, I64, P, I64, I64, P, P, I64, P, P, I64, P, I32, P]),
+    "flint_kv_free": (I32, [P, I64, P, I64, I64, P, P, I64, P, I64, P, I32, P]),
+    "flint_kv_compact": (I32, [P, I64, I64, I64, I64, P, I64, P, I64, I64, P, I64, P, P, P, I32, P]),
 }
 
 
@@ -179,6 +190,8 @@ def workspace(device: torch.device, kind: str, nbytes: int) -> torch.Tensor:
 # ---------------------------------------------------------------------------------------------------------
 STATUS_BITS = {1: "a bounded wait timed out (that launch's outputs are invalid)", 2: "a routed expert id was out "
                "of range (clamped)", 4: "a sequence was longer than its block table (clamped)"}
+_PAGES_BITS = {4: "a stream, length, page or table did not fit (that request was left out)", 8: "fewer pages were free "
+               "than asked for (that request was left out)"}
 _ALIGN_BITS = {1: "an expert id was out of range or sorted_ids was too small"}
 
 
@@ -191,7 +204,7 @@ def _status_kind(name: str) -> int | None:
     for prefix, kind in (("moe_fused_", 2), ("moe_block_", 3), ("attn_block_", 5)):
         if name.startswith(prefix):
             return kind
-    return {"attn_proj": 4, "decode_attention": 6}.get(name)
+    return {"attn_proj": 4, "decode_attention": 6, "paged_attention": 7, "kv_pages": 8}.get(name)
 
 
 def _status_offset(name: str) -> int | None:
@@ -202,7 +215,7 @@ def _status_offset(name: str) -> int | None:
 
 
 def describe_status(name: str, bits: int) -> str:
-    table = _ALIGN_BITS if name == "align_status" else STATUS_BITS
+    table = {"align_status": _ALIGN_BITS, "kv_pages": _PAGES_BITS}.get(name, STATUS_BITS)
     parts = [text for bit, text in table.items() if bits & bit]
     rest = bits & ~sum(table)
     return ", ".join(parts + ([f"bits {rest:#x}"] if rest else []))

@@ -172,6 +172,8 @@ extern "C" int64_t flint_workspace_status_offset(int kind) {
     case FLINT_WS_ATTN_PROJ: return status_offset_attn_proj();
     case FLINT_WS_ATTN_BLOCK: return status_offset_attn_block();
     case FLINT_WS_DECODE_ATTENTION: return status_offset_decode_attention();
+    case FLINT_WS_PAGED_ATTENTION: return status_offset_paged_attention();
+    case FLINT_WS_KV_PAGES: return status_offset_kv_pages();
     default: return -1;
   }
 }

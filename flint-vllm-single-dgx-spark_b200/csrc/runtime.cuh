@@ -28,6 +28,8 @@ int64_t status_offset_moe_block();
 int64_t status_offset_attn_proj();
 int64_t status_offset_attn_block();
 int64_t status_offset_decode_attention();
+int64_t status_offset_paged_attention();
+int64_t status_offset_kv_pages();
 
 // Every kernel runs with the maximum shared-memory carveout, so consecutive kernels of a decode step never make an
 // SM re-partition L1 / shared memory between them.  Set once per (kernel, device).

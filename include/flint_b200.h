@@ -80,12 +80,16 @@ enum {
   FLINT_WS_MOE_BLOCK = 3,         /* flint_moe_block (+ _ep, _peer) */
   FLINT_WS_ATTN_PROJ = 4,         /* flint_attn_qkv, flint_attn_o */
   FLINT_WS_ATTN_BLOCK = 5,        /* flint_attn_block */
-  FLINT_WS_DECODE_ATTENTION = 6   /* flint_decode_attention */
+  FLINT_WS_DECODE_ATTENTION = 6,  /* flint_decode_attention */
+  FLINT_WS_PAGED_ATTENTION = 7,   /* flint_prefill_attention, flint_shared_prefix_attention */
+  FLINT_WS_KV_PAGES = 8           /* flint_kv_* */
 };
 enum {
   FLINT_STATUS_WAIT_TIMEOUT = 1,  /* a bounded wait gave up: that launch's outputs are invalid */
   FLINT_STATUS_BAD_EXPERT = 2,    /* a routed expert id outside 0..E-1 (clamped) */
-  FLINT_STATUS_BAD_SEQUENCE = 4   /* a sequence longer than its block table (clamped to the table) */
+  FLINT_STATUS_BAD_SEQUENCE = 4,  /* a sequence longer than its block table (clamped to the table); of the page
+                                     operations: a stream, length, page or table that does not fit (left out) */
+  FLINT_STATUS_NO_PAGES = 8       /* a page operation asked for more pages than are free (that request is left out) */
 };
 /* Byte offset of the status word inside a workspace of `kind`, or -1 for an unknown kind (no GPU needed). */
 int64_t flint_workspace_status_offset(int kind);
@@ -505,6 +509,72 @@ int flint_moe_grouped_down(const void* ah, const int32_t* shift, const int32_t* 
                            const int32_t* num_tokens_post_pad, int64_t numel, int64_t topk, int64_t E, const void* w2,
                            const void* s2, const float* g2, int64_t H, int64_t I, int64_t max_blocks, void* y,
                            void* workspace, int tensor_cores, int pdl, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Prompts and shared prompts over the paged KV cache.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* Causal grouped-query attention of packed query tokens over the paged cache: whole prompts, chunks of prompts behind
+ * what is cached already, or a few drafted tokens.  q bf16 [tokens, num_q_heads, 128] (row stride q_stride_t elements,
+ * heads contiguous); kv_cache, block_tables and sinks as for flint_decode_attention.  cu_seqlens int32 [batch + 1]: the
+ * query tokens of sequence b are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (none: b is skipped); seq_lens int32 [batch]:
+ * the tokens of b in the cache, its queries' own keys included, so query i of n sits at position p = seq_lens[b] - n + i.
+ * It sees the keys max(0, p - window + 1) .. p (window 0: all up to p); a query that sees none (p < 0) gives zeros.
+ * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written.  Slots of the cache that no
+ * query sees may hold anything, NaN and infinities too.  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache
+ * 16-byte aligned, strides multiples of 8 elements.  workspace: flint_prefill_attention_workspace_bytes(). */
+int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads);
+int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_cache, int64_t num_blocks,
+                            int64_t num_kv_heads, int64_t stride_block, int64_t stride_head, const int32_t* block_tables,
+                            int64_t bt_stride, int64_t max_blocks, const int32_t* cu_seqlens, const int32_t* seq_lens,
+                            const float* sinks, int64_t window, float scale, int64_t batch, int64_t tokens,
+                            int64_t num_q_heads, void* out, int64_t out_stride_t, void* workspace, int pdl, void* stream);
+
+/* flint_decode_attention for streams whose block tables begin with the same pages, which are read once for all of them.
+ * group_starts int32 [groups + 1] (rising from 0 to batch): group g is the streams group_starts[g] ..
+ * group_starts[g + 1] - 1; prefix_lens int32 [groups]: the tokens whose pages its streams share (a page that is not full
+ * is not counted as shared; 0: none), named by the table of the group's first stream.  seq_lens[b] counts the prefix
+ * and the current token; 0 gives zeros.  Other arguments as above, q and out [batch, num_q_heads, 128]. */
+int64_t flint_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads,
+                                                      int64_t num_kv_heads);
+int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, const void* kv_cache, int64_t num_blocks,
+                                  int64_t num_kv_heads, int64_t stride_block, int64_t stride_head,
+                                  const int32_t* block_tables, int64_t bt_stride, int64_t max_blocks,
+                                  const int32_t* seq_lens, const int32_t* group_starts, const int32_t* prefix_lens,
+                                  int64_t groups, const float* sinks, int64_t window, float scale, int64_t batch,
+                                  int64_t num_q_heads, void* out, int64_t out_stride_b, void* workspace, int pdl,
+                                  void* stream);
+
+/* Pages of the cache as a pool that streams share.  The cache of all layers is one bf16 tensor [layers, blocks,
+ * num_kv_heads, 16, 256] (a page [num_kv_heads, 16, 256] contiguous; stride_layer / stride_block in elements, multiples
+ * of 8; kv 16-byte aligned).  The state is device memory of the caller: ref int32 [blocks], how many streams hold a page
+ * (0: free); block_tables int32 [num_streams, max_blocks], -1 behind a stream's pages; num_pages and seq_lens int32
+ * [num_streams].  An empty pool is all zeros with tables of -1.  Pages are taken from the lowest free ids in the order
+ * of the call's streams, so the same state gives the same pages.  streams / src / dst / lens are device int32 [n], n and
+ * num_streams up to 4,096.  A request that does not fit (an id out of range, a stream named twice: the first stands; a
+ * length behind the table; too few free pages) is left out whole and recorded in the status word.
+ *   flint_kv_reserve: stream streams[i] gets pages until it has room for lens[i] tokens (never fewer than it has)
+ *   flint_kv_fork:    empty stream dst[i] (num_pages 0) becomes a copy of src[i]: full pages shared, the last page, if
+ *                     not full, copied in every layer into a page of its own; pages reserved ahead are not inherited
+ *   flint_kv_free:    streams give their pages back
+ *   flint_kv_compact: the used pages behind the first `live` (their number) move, in rising order, to the free ids among
+ *                     the first `live`; tables follow.  remap int32 [blocks]: where a used page is now, -1: free
+ * workspace: flint_kv_pages_workspace_bytes(blocks), one for all four. */
+int64_t flint_kv_pages_workspace_bytes(int64_t blocks);
+int flint_kv_reserve(int32_t* ref, int64_t blocks, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks,
+                     int32_t* num_pages, int64_t num_streams, const int32_t* streams, const int32_t* lens, int64_t n,
+                     void* workspace, int pdl, void* stream);
+int flint_kv_fork(void* kv, int64_t layers, int64_t num_kv_heads, int64_t stride_layer, int64_t stride_block, int32_t* ref,
+                  int64_t blocks, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks, int32_t* seq_lens,
+                  int32_t* num_pages, int64_t num_streams, const int32_t* src, const int32_t* dst, int64_t n,
+                  void* workspace, int pdl, void* stream);
+int flint_kv_free(int32_t* ref, int64_t blocks, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks,
+                  int32_t* seq_lens, int32_t* num_pages, int64_t num_streams, const int32_t* streams, int64_t n,
+                  void* workspace, int pdl, void* stream);
+int flint_kv_compact(void* kv, int64_t layers, int64_t num_kv_heads, int64_t stride_layer, int64_t stride_block,
+                     int32_t* ref, int64_t blocks, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks,
+                     int32_t* num_pages, int64_t num_streams, int32_t* remap, int32_t* live, void* workspace, int pdl,
+                     void* stream);
 
 #ifdef __cplusplus
 }
