@@ -204,7 +204,7 @@ def _status_kind(name: str) -> int | None:
     for prefix, kind in (("moe_fused_", 2), ("moe_block_", 3), ("attn_block_", 5)):
         if name.startswith(prefix):
             return kind
-    return {"attn_proj": 4, "decode_attention": 6, "paged_attention": 7, "kv_pages": 8}.get(name)
+    return {"attn_proj": 4, "decode_attention": 6, "paged_attention": 16, "kv_pages": 17}.get(name)
 
 
 def _status_offset(name: str) -> int | None:

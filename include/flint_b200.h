@@ -81,8 +81,8 @@ enum {
   FLINT_WS_ATTN_PROJ = 4,         /* flint_attn_qkv, flint_attn_o */
   FLINT_WS_ATTN_BLOCK = 5,        /* flint_attn_block */
   FLINT_WS_DECODE_ATTENTION = 6,  /* flint_decode_attention */
-  FLINT_WS_PAGED_ATTENTION = 7,   /* flint_prefill_attention, flint_shared_prefix_attention */
-  FLINT_WS_KV_PAGES = 8           /* flint_kv_* */
+  FLINT_WS_PAGED_ATTENTION = 16,  /* flint_prefill_attention, flint_shared_prefix_attention */
+  FLINT_WS_KV_PAGES = 17          /* flint_kv_* */
 };
 enum {
   FLINT_STATUS_WAIT_TIMEOUT = 1,  /* a bounded wait gave up: that launch's outputs are invalid */
