@@ -204,7 +204,8 @@ def _status_kind(name: str) -> int | None:
     for prefix, kind in (("moe_fused_", 2), ("moe_block_", 3), ("attn_block_", 5)):
         if name.startswith(prefix):
             return kind
-    return {"attn_proj": 4, "decode_attention": 6, "paged_attention": 16, "kv_pages": 17}.get(name)
+    return {"attn_proj": 4, "decode_attention": 6, "prefill_attention": 16, "shared_prefix_attention": 16,
+            "kv_pages": 17}.get(name)
 
 
 def _status_offset(name: str) -> int | None:

@@ -1,14 +1,31 @@
 // Attention of many query rows over the paged KV cache: a prompt (or a chunk of one, or drafted tokens) read causally
-// (flint_prefill_attention), and decode streams whose block tables begin with the same pages
-// (flint_shared_prefix_attention).
+// (flint_prefill_attention), and decode streams whose block tables begin with the same pages, which are read once for all
+// of them (flint_shared_prefix_attention).
 //
 // KV cache: HND bf16 [num_blocks, num_kv_heads, 16, 2 * 128], K in the first 128 columns of a token's row, V in the rest.
-// A tile is up to 64 query rows of one KV head: consecutive tokens of one sequence, each with its G query heads (row =
-// token * G + head), so that the group reads its keys once.  With c = scale * log2(e), a row at position p over the keys
-// max(0, p - window + 1) .. p keeps the running maximum m and, in 32 bits, l = sum 2^(c (s - m)) and o = sum 2^(..) v;
-// the probabilities are rounded to bf16 for the product with V only (l sums the unrounded ones, as the decode attention
-// does).  A sink adds 2^(sink log2 e - c m) to l.  A row without keys gives zeros.  Cache slots that no row may see are
-// never multiplied: their scores are replaced, their V rows read as zero.
+// With c = scale * log2(e), a row over its visible keys keeps a reference m, l = sum 2^(c (s - m)) and o = sum 2^(..) v in
+// 32 bits; the probabilities are rounded to bf16 for the product with V only (l sums the unrounded ones, as the decode
+// attention does).  Results over disjoint keys join as m = max m_k, l = sum l_k 2^(c (m_k - m)), o likewise.  A sink adds
+// 2^(sink log2 e - c m) to l.  A row without keys gives zeros.
+//
+// Work.  An item is one KV head and up to two row tiles of 128 rows: floor(128 / G) consecutive query tokens (or streams)
+// with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys,
+// doubled for two tiles, and a constant), the line is cut into equal shares, one per SM: a long prompt's items and a few
+// rows on a long cache are both split evenly, and where a cut falls into an item its parts leave (m, l, o) in the
+// workspace and a second launch joins them in the order of the keys.
+//   an item of two tiles: both tiles multiply the same keys; one's softmax runs under the other's products
+//   an item of one tile:  its keys are dealt to the two halves of the block in turn, and joined at the end
+//
+// Block: two softmax groups of 4 warps (a thread per row), a warp each for TMA, for the MMAs and for cutting the items.
+// Keys come 128 at a time: 8 pages, one TMA box of 16 tokens x 64 columns per half of K or V, 128-byte swizzle, into a ring
+// of four 32 KB slots.  S = Q K^T (both from shared memory) and O += P V (P from tensor memory, where it overwrites its S;
+// V as it lies, tokens as the K dimension) are tcgen05 products of 128 x 128 x 128, issued by one lane.  The MMAs of one
+// thread run in order, so when S of a step has come, the O of the step before is complete: the softmax group may rescale
+// it.  It does so only when a row's maximum rises by more than 2^8 over the reference, which the first steps do.
+// Slots that no row may see are never multiplied: a page that an item does not reach is read out of bounds (zeros), and
+// its last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too.
+#include <limits.h>
+
 #include "common.cuh"
 #include "runtime.cuh"
 #include "tma.cuh"
@@ -17,205 +34,849 @@ namespace flint {
 
 constexpr int kPaD = 128;
 constexpr int kPaPage = 16;
-constexpr int kPaRows = 64;                    // query rows of a tile
-constexpr int kPaKeys = 64;                    // keys of a step
-constexpr int kPaLd = kPaD + 8;                // halves of a staged row: 16-byte units of 8 rows fall in 8 bank groups
+constexpr int kPaM = 128;                      // rows of a tile
+constexpr int kPaKeys = 128;                   // keys of a step
+constexpr int kPaSlots = 4;                    // ring slots of 128 keys x 128 columns (K or V)
+constexpr int kPaSlotBytes = kPaKeys * kPaD * 2;
+constexpr int kPaHalf = kPaSlotBytes / 2;      // 64 columns
+constexpr int kPaPageHalf = kPaPage * 128;     // a page's 64 columns
+constexpr int kPaQueue = 4;                    // items cut ahead
+constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA, items, one idle
+constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
+constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
+constexpr int kPaFixed = 160;                  // cost of an item beside its keys, in keys of one tile
+constexpr int kPaLeast = 256;                  // least share of a block, in keys of one tile
 constexpr unsigned STATUS_BAD_SEQ = 4u;
+constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 64 * 4;
 
 struct PagedAttnWorkspace {
   unsigned status;
   unsigned pad[31];
 };
 
+// Where the parts of a token's result are: with blocks first .. last (counted from 1), or one of the values below in
+// `first`.  0 in `first`: nothing to join, what the join leaves behind for prompts (whose spare rows have no item).
+struct PaRecord {
+  int first, last;
+  int tok0;                                    // the item's first token
+  int prefix;                                  // of a stream's own keys: its group's prefix has a record too
+};
+enum { PA_FINAL = -1, PA_HOME = -2, PA_NONE = -3 };
+
 struct PagedAttnArgs {
-  const bf16* q;
-  int64_t q_stride;                            // elements between tokens
-  const bf16* kv;
-  int64_t stride_block, stride_head;           // elements
-  int64_t num_blocks;
-  const int* block_tables;
   int64_t bt_stride;
+  const int* block_tables;
   int max_blocks;
-  const int* cu_seqlens;                       // [batch + 1], or null: sequence b is the one token b
+  const int* cu_seqlens;                       // prompts: [batch + 1]
   const int* seq_lens;
-  const int *group_starts, *prefix_lens;       // shared prefixes only
+  const int *group_starts, *prefix_lens;       // shared prefixes
   int groups;
   const float* sinks;
-  int window, batch, tokens, Hkv, G;
+  int window, batch, tokens, Hkv, G, num_blocks;
   float c;
   bf16* out;
   int64_t out_stride;
   PagedAttnWorkspace* ws;
+  PaRecord* rec;                               // [tokens][Hkv] (shared: own keys, then [batch][Hkv] prefixes)
+  float2 *ml, *home_ml;                        // (m, l): slots [2 x blocks][256 rows], homes [2][batch][Hq]
+  float4 *o, *home_o;                          // the same rows' o: slots [32 quads of columns][256 rows], homes [row][32]
 };
 
-__device__ __forceinline__ void pa_ldsm(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+struct PaItem {
+  int tok0, ntok;                              // query tokens (streams)
+  int h, table;                                // KV head, row of the block tables
+  int begin, end;                              // keys; begin at a page
+  int j0, j1;                                  // steps of this part
+  int pos0;                                    // position of the first token; prefix: -1
+  int dual;
+  int out;                                     // slot, PA_HOME or PA_FINAL
+  int home;                                    // 0: own keys, 1: prefix
+};
+
+// ---- tensor memory and MMA ----
+__device__ __forceinline__ void pa_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
 }
-__device__ __forceinline__ void pa_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+__device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void pa_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Shared-memory operand, 128-byte swizzle (rows of 128 B, 8 rows to 1,024 B).  K along the row: 8-row groups 1,024 B apart.
+// K down the rows (V): 8 rows of K 1,024 B apart, the next 64 columns `lead` bytes on.
+__device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulator, bf16 operands, N = 128, M = 128
+constexpr uint32_t kPaIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+constexpr uint32_t kPaIdescPV = kPaIdescQK | (1u << 16);          // B with K down the rows
+__device__ __forceinline__ void pa_mma_qk(uint32_t d, uint32_t q, uint32_t k) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {                                   // 16 columns of Q and K at a time
+    const uint32_t off = (i >> 2) * kPaHalf + (i & 3) * 32;
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(pa_desc(q + off, 16)),
+        "l"(pa_desc(k + off, 16)), "r"(kPaIdescQK), "r"(i > 0 ? 1u : 0u)
+        : "memory");
+  }
+}
+__device__ __forceinline__ void pa_mma_pv(uint32_t d, uint32_t p, uint32_t v, bool add) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)                                     // 16 keys at a time: 8 columns of P, 16 rows of V
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(p + 8 * i),
+        "l"(pa_desc(v + i * 2048, kPaHalf)), "r"(kPaIdescPV), "r"(add || i > 0 ? 1u : 0u)
+        : "memory");
+}
+// TMA boxes without an L2 hint: other blocks read the same keys
+__device__ __forceinline__ void pa_tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void pa_tma_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+          "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ float pa_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
-  __shared__ __align__(16) bf16 sk[kPaKeys][kPaLd], sv[kPaKeys][kPaLd];
+// A wait for the phase of the given parity that gives up after two seconds, or as soon as another warp of the block has.
+constexpr unsigned long long kPaWaitNs = 2000000000ull;
+__device__ __forceinline__ unsigned long long pa_now() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __noinline__ bool pa_wait_long(uint64_t* bar, unsigned parity, volatile int* failed, unsigned* status) {
+  const unsigned long long t0 = pa_now();
+  while (!*failed) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (pa_now() - t0 > kPaWaitNs) {
+      *failed = 1;
+      atomicOr(status, STATUS_WAIT_TIMEOUT);
+    }
+  }
+  return false;
+}
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile int* failed, unsigned* status) {
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return pa_wait_long(bar, parity, failed, status);
+}
+
+// ---- the items ----
+// sum over i < k of max(0, a + i * t)
+__device__ __forceinline__ long long pa_ramp(long long a, long long t, long long k) {
+  long long i0 = a < 0 ? (-a + t - 1) / t : 0;
+  if (i0 > k) i0 = k;
+  return a * (k - i0) + t * ((k - 1) * k - (i0 - 1) * i0) / 2;
+}
+
+// A run of row tiles on one line: a prompt's, a group's (its prefix) or a stream's own keys.  Every field is the same for
+// all blocks, so that all of them cut the line at the same places.
+struct PaSegment {
+  int tok0, ntok;                              // its tokens (streams)
+  int table;
+  int pos0;                                    // position of the first token; prefix: -1
+  int lo, hi;                                  // keys outside [lo, hi) are another segment's
+  int home;
+  long long cost;                              // of one KV head
+};
+
+struct PaLine {
+  const PagedAttnArgs& a;
+  const bool shared;
+  const int per, tile;                         // tokens of a row tile, of an item
+
+  __device__ PaLine(const PagedAttnArgs& args) : a(args), shared(args.group_starts != nullptr), per(kPaM / args.G), tile(2 * per) {}
+  __device__ int segments() const { return shared ? a.groups + a.batch : a.batch; }
+  __device__ void complain(bool bad) const {
+    if (bad && blockIdx.x == 0) atomicOr(&a.ws->status, STATUS_BAD_SEQ);
+  }
+  __device__ int length(int b) const {
+    const int most = a.max_blocks * kPaPage, n = a.seq_lens[b];
+    complain(n > most);
+    return max(0, min(n, most));
+  }
+  // streams and shared tokens of group g; a group of one shares nothing
+  __device__ int group(int g, int* first, int* prefix) const {
+    const int s0 = a.group_starts[g], s1 = a.group_starts[g + 1], n = a.prefix_lens[g];
+    const bool bad = s0 < 0 || s1 < s0 || s1 > a.batch || n < 0 || n > a.max_blocks * kPaPage;
+    complain(bad);
+    *first = s0;
+    *prefix = bad || s1 - s0 < 2 ? 0 : n & ~(kPaPage - 1);
+    return bad ? 0 : s1 - s0;
+  }
+  __device__ int prefix_of(int b) const {
+    int lo = 0, hi = a.groups - 1;             // the last group that starts at or before b
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.group_starts[mid] <= b) lo = mid; else hi = mid - 1;
+    }
+    int first, prefix;
+    const int n = group(lo, &first, &prefix);
+    return b >= first && b < first + n ? prefix : 0;
+  }
+  __device__ PaSegment segment(int i) const {
+    PaSegment s = {};
+    if (i >= segments()) return s;
+    if (!shared) {
+      const int first = a.cu_seqlens[i], next = a.cu_seqlens[i + 1];
+      const bool bad = first < 0 || next < first || next > a.tokens;
+      complain(bad);
+      s.tok0 = first, s.ntok = bad ? 0 : next - first, s.table = i;
+      if (s.ntok) s.hi = length(i);
+      s.pos0 = s.hi - s.ntok;
+      complain(a.seq_lens[i] < 0);
+    } else if (i < a.groups) {
+      int prefix;
+      s.ntok = group(i, &s.tok0, &prefix);
+      s.table = s.tok0, s.pos0 = -1, s.home = 1, s.hi = prefix;
+      if (!prefix) s.ntok = 0;
+    } else {
+      const int b = i - a.groups;
+      s.tok0 = b, s.ntok = 1, s.table = b;
+      s.hi = length(b);
+      s.lo = min(prefix_of(b), s.hi), s.pos0 = s.hi - 1;
+    }
+    s.cost = upto(s, (s.ntok + tile - 1) / tile);
+    return s;
+  }
+  __device__ int tokens_of(const PaSegment& s, int i) const { return min(tile, s.ntok - i * tile); }
+  // keys that item i is taken to cost
+  __device__ long long keys(const PaSegment& s, int i) const {
+    if (s.home) return a.window > 0 ? min(s.hi, a.window) : s.hi;
+    const long long p = (long long)s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
+    return max(0ll, e) - max((long long)s.lo, b) > 0 ? max(0ll, e) - max((long long)s.lo, b) : 0;
+  }
+  __device__ long long weight(const PaSegment& s, int i) const { return (tokens_of(s, i) > per ? 2 : 1) * keys(s, i); }
+  // cost of the items before item k
+  __device__ long long upto(const PaSegment& s, int k) const {
+    const int m = (s.ntok + tile - 1) / tile;
+    if (k <= 0 || m == 0) return 0;
+    const long long whole = min(k, m - 1);     // the last item may be shorter
+    long long w;
+    if (s.home) w = 2 * whole * keys(s, 0);
+    else {
+      w = pa_ramp((long long)s.pos0 + tile, tile, whole);
+      if (a.window > 0) w -= pa_ramp((long long)s.pos0 - a.window + 1, tile, whole);
+      w *= 2;
+    }
+    if (k >= m) w += weight(s, m - 1);
+    return w + (long long)kPaFixed * min(k, m);
+  }
+};
+static_assert(kPaFixed > 0, "every item has a place on the line");
+
+__global__ void __launch_bounds__(kPaThreads, 1)
+paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const PagedAttnArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;                                             // two Q tiles, each two halves of 64 columns
+  uint8_t* ring = sq + 2 * kPaSlotBytes;
+  float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 64 columns of o between the halves
+  __shared__ PaItem items[kPaQueue];
+  __shared__ __align__(8) uint64_t b_item[kPaQueue], b_item_free[kPaQueue], b_full[kPaSlots], b_empty[kPaSlots], b_q, b_q_free,
+      b_s[2], b_p[2], b_o[2], b_hand, b_take;
+  __shared__ float2 s_ml[kPaM];
+  __shared__ uint32_t s_taddr;
+  __shared__ int s_failed;                                        // a wait ran out: every warp leaves
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned* status = &a.ws->status;
+  if (tid == 0) {
+    s_failed = 0;
+    for (int i = 0; i < kPaQueue; ++i) {
+      mbar_init(&b_item[i], 1);
+      mbar_init(&b_item_free[i], 10);                             // 8 softmax warps, TMA, MMA
+    }
+    for (int i = 0; i < kPaSlots; ++i) {
+      mbar_init(&b_full[i], 1);
+      mbar_init(&b_empty[i], 1);
+    }
+    mbar_init(&b_q, 1);
+    mbar_init(&b_q_free, 1);
+    mbar_init(&b_hand, 4);
+    mbar_init(&b_take, 4);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&b_s[t], 1);
+      mbar_init(&b_p[t], 4);
+      mbar_init(&b_o[t], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_taddr)),
+                 "r"((uint32_t)kPaTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pa_fence_before();
+  __syncthreads();
+  pa_fence_after();
+  const uint32_t tmem = s_taddr;
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g4 = lane >> 2, t4 = lane & 3;
-  const int h = blockIdx.y, tile_tokens = kPaRows / a.G;
-  if (blockIdx.x == 0 && h == 0)
-    for (int i = tid; i < a.groups; i += 128) {
-      const int s0 = a.group_starts[i], s1 = a.group_starts[i + 1], n = a.prefix_lens[i];
-      if (s0 < 0 || s1 < s0 || s1 > a.batch || n < 0 || n > a.max_blocks * kPaPage) atomicOr(&a.ws->status, STATUS_BAD_SEQ);
-    }
-  // the tile's sequence and first token: sequences take ceil(n / tile_tokens) tiles each, in order
-  int b = 0, first = 0, n = 0, t0 = 0;
-  {
-    int left = blockIdx.x;
-    for (; b < a.batch; ++b) {
-      first = a.cu_seqlens ? a.cu_seqlens[b] : b;
-      n = (a.cu_seqlens ? a.cu_seqlens[b + 1] : b + 1) - first;
-      if (first < 0 || n < 0 || first + n > a.tokens) {
-        if (tid == 0) atomicOr(&a.ws->status, STATUS_BAD_SEQ);
-        n = 0;
-      }
-      const int tiles = (n + tile_tokens - 1) / tile_tokens;
-      if (left < tiles) break;
-      left -= tiles;
-    }
-    if (b == a.batch) return;
-    t0 = left * tile_tokens;
-  }
-  int len = a.seq_lens[b];
-  if (len > a.max_blocks * kPaPage) {
-    len = a.max_blocks * kPaPage;
-    if (tid == 0) atomicOr(&a.ws->status, STATUS_BAD_SEQ);
-  }
-  const int rows = min(tile_tokens, n - t0) * a.G;
-  const int pos0 = len - n + t0;                                  // position of the tile's first token
-  const int pos_last = pos0 + min(tile_tokens, n - t0) - 1;
-  const int end = max(0, pos_last + 1);
-  const int begin = a.window > 0 ? max(0, pos0 - a.window + 1) & ~(kPaPage - 1) : 0;
-
-  // this thread's rows of the warp's 16: r0 = 16 warp + g4 and r0 + 8
-  int lo[2], hi[2];
-  const bf16* qrow[2];
-  bool valid[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 16 * warp + g4 + 8 * i;
-    valid[i] = r < rows;
-    const int tok = r / a.G, p = pos0 + tok;
-    hi[i] = valid[i] ? p + 1 : 0;
-    lo[i] = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    qrow[i] = a.q + (int64_t)(first + t0 + tok) * a.q_stride + (h * a.G + r - tok * a.G) * kPaD;
-  }
-  uint32_t qa[8][4];
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      qa[kk][i] = valid[i & 1] ? *reinterpret_cast<const uint32_t*>(qrow[i & 1] + 16 * kk + 8 * (i >> 1) + 2 * t4) : 0u;
-  float o[16][4];
-#pragma unroll
-  for (int d = 0; d < 16; ++d)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  for (int k0 = begin; k0 < end; k0 += kPaKeys) {
-    __syncthreads();
-    for (int u = tid; u < kPaKeys * 32; u += 128) {
-      const int key = u >> 5, unit = u & 31;                      // 16-byte units of a token's K | V row
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (k0 + key < end) {
-        const int blk = a.block_tables[(int64_t)b * a.bt_stride + (k0 + key) / kPaPage];
-        if (blk >= 0 && blk < a.num_blocks)
-          v = *reinterpret_cast<const uint4*>(a.kv + blk * a.stride_block + h * a.stride_head +
-                                              ((k0 + key) & (kPaPage - 1)) * 2 * kPaD + unit * 8);
-      }
-      *reinterpret_cast<uint4*>(unit < 16 ? &sk[key][unit * 8] : &sv[key][(unit - 16) * 8]) = v;
-    }
-    __syncthreads();
-    float s[8][4];
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-    const int mat = lane >> 3, r8 = lane & 7;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk)
-#pragma unroll
-      for (int np = 0; np < 4; ++np) {
-        uint32_t kf[4];
-        pa_ldsm(smem_u32(&sk[16 * np + 8 * (mat >> 1) + r8][16 * kk + 8 * (mat & 1)]), kf);
-        mma_bf16(s[2 * np], qa[kk], kf[0], kf[1]);
-        mma_bf16(s[2 * np + 1], qa[kk], kf[2], kf[3]);
-      }
-    float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 8 * nt + 2 * t4 + (e & 1), i = e >> 1;
-        if (key >= hi[i] || key < lo[i]) s[nt][e] = -INFINITY;
-        top[i] = fmaxf(top[i], s[nt][e]);
-      }
-    float base[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      const float mn = fmaxf(m[i], top[i]);
-      base[i] = mn == -INFINITY ? 0.f : mn * a.c;
-      const float alpha = m[i] == -INFINITY ? 0.f : exp2f(m[i] * a.c - base[i]);
-      m[i] = mn;
-      l[i] *= alpha;
-#pragma unroll
-      for (int d = 0; d < 16; ++d) {
-        o[d][2 * i] *= alpha;
-        o[d][2 * i + 1] *= alpha;
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[nt][e] = exp2f(s[nt][e] * a.c - base[e >> 1]);
-        l[e >> 1] += s[nt][e];
-      }
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {                              // 16 keys at a time
-      const uint32_t pa[4] = {pa_pack(s[2 * kt][0], s[2 * kt][1]), pa_pack(s[2 * kt][2], s[2 * kt][3]),
-                              pa_pack(s[2 * kt + 1][0], s[2 * kt + 1][1]), pa_pack(s[2 * kt + 1][2], s[2 * kt + 1][3])};
-#pragma unroll
-      for (int dp = 0; dp < 8; ++dp) {
-        uint32_t vf[4];
-        pa_ldsm_t(smem_u32(&sv[16 * kt + 8 * (mat & 1) + r8][16 * dp + 8 * (mat >> 1)]), vf);
-        mma_bf16(o[2 * dp], pa, vf[0], vf[1]);
-        mma_bf16(o[2 * dp + 1], pa, vf[2], vf[3]);
-      }
-    }
-  }
   pdl_trigger();
+
+  if (warp == 10) {
+    // ---- items: this block's share of the line ----
+    const PaLine line(a);
+    const int nseg = line.segments();
+    long long total = 0;
+    for (int i0 = 0; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (!valid[i]) continue;
-    const int r = 16 * warp + g4 + 8 * i, tok = r / a.G, qh = h * a.G + r - tok * a.G;
-    float den = l[i];
-    if (a.sinks && m[i] != -INFINITY) den += exp2f(a.sinks[qh] * kPaLog2e - m[i] * a.c);
-    const float inv = m[i] == -INFINITY ? 0.f : 1.0f / den;
-    bf16* dst = a.out + (int64_t)(first + t0 + tok) * a.out_stride + qh * kPaD;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const long long shares = max(1ll, min((long long)gridDim.x, total / kPaLeast));
+    auto cut = [&](long long c) { return c >= shares ? total : total * c / shares; };
+    const long long x0 = cut(blockIdx.x), x1 = blockIdx.x < shares ? cut(blockIdx.x + 1) : x0;
+    long long at = 0;                                             // cost of the segments before the chunk's lane 0
+    int n_items = 0;
+    bool ok = true;
+    for (int i0 = 0; i0 < nseg && at < x1 && ok; i0 += 32) {
+      const PaSegment mine = line.segment(i0 + lane);
+      long long cum = mine.cost * a.Hkv;                          // inclusive scan over the lanes
 #pragma unroll
-    for (int d = 0; d < 16; ++d)
-      *reinterpret_cast<uint32_t*>(dst + 8 * d + 2 * t4) = pa_pack(o[d][2 * i] * inv, o[d][2 * i + 1] * inv);
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, cum, o);
+        if (lane >= o) cum += y;
+      }
+      const long long chunk = __shfl_sync(0xffffffffu, cum, 31);
+      if (at + chunk <= x0) {
+        at += chunk;
+        continue;
+      }
+      for (int k = 0; k < 32 && ok; ++k) {
+        PaSegment s;
+        s.tok0 = __shfl_sync(0xffffffffu, mine.tok0, k);
+        s.ntok = __shfl_sync(0xffffffffu, mine.ntok, k);
+        s.table = __shfl_sync(0xffffffffu, mine.table, k);
+        s.pos0 = __shfl_sync(0xffffffffu, mine.pos0, k);
+        s.lo = __shfl_sync(0xffffffffu, mine.lo, k);
+        s.hi = __shfl_sync(0xffffffffu, mine.hi, k);
+        s.home = __shfl_sync(0xffffffffu, mine.home, k);
+        s.cost = __shfl_sync(0xffffffffu, mine.cost, k);
+        const long long seg0 = at + __shfl_sync(0xffffffffu, cum, k) - s.cost * a.Hkv;
+        if (s.cost == 0 || seg0 + s.cost * a.Hkv <= x0) continue;
+        if (seg0 >= x1) break;
+        const int m = (s.ntok + line.tile - 1) / line.tile;
+        int h = 0, i = 0;
+        if (x0 > seg0) {                                          // the first item that the share touches
+          h = (int)((x0 - seg0) / s.cost);
+          const long long y = (x0 - seg0) % s.cost;
+          int hi = m - 1;
+          while (i < hi) {
+            const int mid = (i + hi + 1) >> 1;
+            if (line.upto(s, mid) <= y) i = mid; else hi = mid - 1;
+          }
+        }
+        for (; h < a.Hkv && ok; ++h, i = 0)
+          for (; i < m; ++i) {
+            const long long start = seg0 + h * s.cost + line.upto(s, i), w = line.weight(s, i), stop = start + kPaFixed + w;
+            if (start >= x1) break;
+            PaItem it;
+            it.tok0 = s.tok0 + i * line.tile, it.ntok = line.tokens_of(s, i), it.h = h, it.table = s.table;
+            it.dual = it.ntok > line.per;
+            it.home = s.home;
+            if (s.home) {                                         // the keys that the tile's streams see of the prefix
+              int lo = INT_MAX, hi = 0;
+              for (int r = lane; r < it.ntok; r += 32) {
+                const int len = line.length(it.tok0 + r);
+                hi = max(hi, len);
+                if (len > 0) lo = min(lo, a.window > 0 ? max(0, len - a.window) : 0);
+              }
+              hi = __reduce_max_sync(0xffffffffu, hi);
+              lo = __reduce_min_sync(0xffffffffu, lo);
+              it.pos0 = -1;
+              it.end = min(s.hi, hi);
+              it.begin = lo < it.end ? lo & ~(kPaPage - 1) : it.end;
+            } else {
+              it.pos0 = s.pos0 + i * line.tile;
+              it.end = max(0, it.pos0 + it.ntok);
+              it.begin = max(s.lo, a.window > 0 ? max(0, it.pos0 - a.window + 1) & ~(kPaPage - 1) : 0);
+              if (it.begin > it.end) it.begin = it.end;
+            }
+            const int steps = (it.end - it.begin + kPaKeys - 1) / kPaKeys;
+            // which steps lie before place x of the line
+            auto before = [&](long long x) -> int {
+              if (x >= stop) return steps;
+              if (x <= start + kPaFixed || w <= 0) return 0;
+              return (int)min((long long)steps, (x - start - kPaFixed) * steps / w);
+            };
+            it.j0 = before(x0), it.j1 = before(x1);
+            PaRecord rec = {PA_NONE, PA_NONE, it.tok0, !s.home && s.lo > 0};
+            bool first = false;                                   // this part writes the record
+            if (steps == 0) {
+              if (start < x0) continue;
+              first = true;
+              it.out = PA_FINAL;
+              if (s.home || rec.prefix) it.out = PA_HOME, rec.first = PA_NONE;
+              else rec.first = PA_FINAL;
+            } else {
+              if (it.j0 == it.j1 && (it.j0 == 0 || it.j0 == steps)) continue;
+              first = it.j0 == 0;
+              if (it.j0 == 0 && it.j1 == steps) {
+                it.out = s.home || rec.prefix ? PA_HOME : PA_FINAL;
+                rec.first = it.out;
+              } else {
+                it.out = 2 * blockIdx.x + (it.j0 == 0);
+                rec.first = blockIdx.x + 1;
+                if (first) {
+                  long long c = blockIdx.x + 1;
+                  while (before(cut(c)) < steps) ++c;
+                  rec.last = (int)c;
+                }
+              }
+            }
+            if (first) {
+              PaRecord* to = a.rec + (s.home ? (int64_t)a.batch * a.Hkv : 0);
+              for (int r = lane; r < it.ntok; r += 32) to[(int64_t)(it.tok0 + r) * a.Hkv + h] = rec;
+            }
+            const int q = n_items % kPaQueue;
+            if (n_items >= kPaQueue && !pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) {
+              items[q] = it;
+              mbar_arrive(&b_item[q]);
+            }
+            __syncwarp();
+            ++n_items;
+          }
+      }
+      at += chunk;
+    }
+    // an item without tokens ends the block
+    const int q = n_items % kPaQueue;
+    if (n_items >= kPaQueue && ok) ok = pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status);
+    if (ok && lane == 0) {
+      items[q].ntok = 0;
+      mbar_arrive(&b_item[q]);
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ---- TMA ----
+    int slot = 0, parity = 1, nq = 0;                             // an empty ring's slots count as released
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+      const PaItem it = items[n % kPaQueue];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
+      if (it.ntok == 0) break;
+      const int steps = it.j1 - it.j0;
+      if (steps == 0) continue;
+      const int* row = a.block_tables + (int64_t)it.table * a.bt_stride;
+      const int pages_end = (it.end + kPaPage - 1) / kPaPage;
+      int held = -1, ids = 0;                                     // table entries of four steps, one per lane
+      auto load = [&](int j, int column) {                        // step j's K (column 0) or V (column 128)
+        const int p0 = it.begin / kPaPage + j * 8;
+        if (held != j >> 2) {
+          held = j >> 2;
+          const int p = it.begin / kPaPage + held * 32 + lane;
+          ids = p < pages_end ? row[p] : a.num_blocks;
+        }
+        const int blk = __shfl_sync(0xffffffffu, ids, (j & 3) * 8 + (lane & 7));
+        if (ok && !pa_wait(&b_empty[slot], (unsigned)parity, &s_failed, status)) ok = false;
+        if (ok) {
+          if (lane == 0) mbar_arrive_expect_tx(&b_full[slot], kPaSlotBytes);
+          __syncwarp();
+          if (lane < 8) {
+            const int left = it.end - (p0 + lane) * kPaPage;      // tokens from this page on
+            const int shift = left > 0 && left < kPaPage ? kPaPage - left : 0;
+            const uint32_t dst = smem_u32(ring + slot * kPaSlotBytes) + lane * kPaPageHalf;
+            pa_tma_4d(dst, &mkv, column, -shift, it.h, blk, &b_full[slot]);
+            pa_tma_4d(dst + kPaHalf, &mkv, column + 64, -shift, it.h, blk, &b_full[slot]);
+          }
+          __syncwarp();
+        }
+        if (++slot == kPaSlots) slot = 0, parity ^= 1;
+      };
+      load(it.j0, 0);
+      if (ok && !pa_wait(&b_q_free, (unsigned)((nq & 1) ^ 1), &s_failed, status)) ok = false;
+      ++nq;
+      if (ok && lane == 0) {
+        const int tiles = it.dual ? 2 : 1, per = kPaM / a.G;
+        mbar_arrive_expect_tx(&b_q, (unsigned)(tiles * 2 * per * a.G * 128));
+        for (int t = 0; t < tiles; ++t)
+          for (int half = 0; half < 2; ++half)
+            pa_tma_3d(smem_u32(sq) + t * kPaSlotBytes + half * kPaHalf, &mq, half * 64, it.h * a.G, it.tok0 + t * per, &b_q);
+      }
+      __syncwarp();
+      if (it.dual) {                                              // K0 V0 K1 V1 ..
+        for (int j = it.j0; j < it.j1; ++j) {
+          if (j > it.j0) load(j, 0);
+          load(j, 128);
+        }
+      } else {                                                    // K0 K1 V0 K2 V1 K3 ..
+        if (steps > 1) load(it.j0 + 1, 0);
+        for (int j = it.j0; j < it.j1; ++j) {
+          load(j, 128);
+          if (j + 2 < it.j1) load(j + 2, 0);
+        }
+      }
+    }
+  } else if (warp == 9) {
+    // ---- MMA ----
+    if (lane == 0) {
+      int slot = 0, parity = 0, p_par[2] = {0, 0}, nq = 0;
+      bool ok = true;
+      const uint32_t s_ring = smem_u32(ring), s_q = smem_u32(sq);
+      auto next = [&]() {                                         // the next slot of the ring, filled
+        const int at = slot;
+        if (ok && !pa_wait(&b_full[at], (unsigned)parity, &s_failed, status)) ok = false;
+        if (++slot == kPaSlots) slot = 0, parity ^= 1;
+        return at;
+      };
+      auto wait_p = [&](int t) {
+        if (ok && !pa_wait(&b_p[t], (unsigned)p_par[t], &s_failed, status)) ok = false;
+        p_par[t] ^= 1;
+        pa_fence_after();
+      };
+      for (int n = 0; ok; ++n) {
+        if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+        const PaItem it = items[n % kPaQueue];
+        mbar_arrive(&b_item_free[n % kPaQueue]);
+        if (it.ntok == 0) break;
+        const int steps = it.j1 - it.j0;
+        if (steps == 0) continue;
+        if (!pa_wait(&b_q, (unsigned)(nq++ & 1), &s_failed, status)) break;
+        pa_fence_after();
+        if (it.dual) {
+          int k = next();
+          for (int t = 0; t < 2 && ok; ++t) {
+            pa_mma_qk(tmem + 128 * t, s_q + t * kPaSlotBytes, s_ring + k * kPaSlotBytes);
+            pa_commit(&b_s[t]);
+          }
+          pa_commit(&b_empty[k]);
+          if (steps == 1) pa_commit(&b_q_free);
+          for (int j = 0; j < steps && ok; ++j) {
+            const int v = next();
+            for (int t = 0; t < 2 && ok; ++t) {
+              wait_p(t);
+              if (!ok) break;
+              pa_mma_pv(tmem + 256 + 128 * t, tmem + 128 * t, s_ring + v * kPaSlotBytes, j > 0);
+              if (t == 1) pa_commit(&b_empty[v]);
+              if (j + 1 < steps) {
+                if (t == 0) k = next();
+                if (!ok) break;
+                pa_mma_qk(tmem + 128 * t, s_q + t * kPaSlotBytes, s_ring + k * kPaSlotBytes);
+                pa_commit(&b_s[t]);
+                if (t == 1) {
+                  pa_commit(&b_empty[k]);
+                  if (j + 2 == steps) pa_commit(&b_q_free);
+                }
+              } else {
+                pa_commit(&b_o[t]);
+              }
+            }
+          }
+        } else {
+          for (int t = 0; t < 2 && t < steps; ++t) {
+            const int k = next();
+            if (!ok) break;
+            pa_mma_qk(tmem + 128 * t, s_q, s_ring + k * kPaSlotBytes);
+            pa_commit(&b_s[t]);
+            pa_commit(&b_empty[k]);
+            if (t + 1 == steps) pa_commit(&b_q_free);
+          }
+          for (int j = 0; j < steps && ok; ++j) {
+            const int t = j & 1, v = next();
+            wait_p(t);
+            if (!ok) break;
+            pa_mma_pv(tmem + 256 + 128 * t, tmem + 128 * t, s_ring + v * kPaSlotBytes, j > 1);
+            pa_commit(&b_empty[v]);
+            if (j + 2 < steps) {
+              const int k = next();
+              if (!ok) break;
+              pa_mma_qk(tmem + 128 * t, s_q, s_ring + k * kPaSlotBytes);
+              pa_commit(&b_s[t]);
+              pa_commit(&b_empty[k]);
+              if (j + 3 == steps) pa_commit(&b_q_free);
+            } else {
+              pa_commit(&b_o[t]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ---- softmax: group t of 128 threads, one row each ----
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
+    int s_par = 0, o_par = 0, handed = 0;                         // handed: halves of o from group 1 to group 0 so far
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+      const PaItem it = items[n % kPaQueue];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
+      if (it.ntok == 0) break;
+      const int per = kPaM / a.G, steps = it.j1 - it.j0;
+      const int tok = row / a.G + (it.dual ? t * per : 0);
+      const int qh = it.h * a.G + row % a.G;
+      const bool valid = row / a.G < per && tok < it.ntok;
+      int lo = 0, hi = 0;                                         // this row's keys
+      if (valid) {
+        if (!it.home) hi = it.pos0 + tok + 1;
+        else hi = max(0, min(a.seq_lens[it.tok0 + tok], a.max_blocks * kPaPage));
+        if (a.window > 0) lo = max(0, hi - a.window);
+        hi = max(0, min(hi, it.end));
+      }
+      float m = -INFINITY, l = 0.f;
+      const int stride = it.dual ? 1 : 2, mine0 = it.dual ? 0 : t;
+      const int last_page = it.end & ~(kPaPage - 1);              // a cut last page: its tokens lie at its slot's end
+      const int shift = it.end > last_page ? kPaPage - (it.end - last_page) : 0;
+      for (int j = mine0; j < steps && ok; j += stride) {
+        if (!pa_wait(&b_s[t], (unsigned)s_par, &s_failed, status)) {
+          ok = false;
+          break;
+        }
+        s_par ^= 1;
+        pa_fence_after();
+        uint32_t r[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pa_ld32(s_col + 32 * q, r + 32 * q);
+        pa_wait_ld();
+        const int k0 = it.begin + (it.j0 + j) * kPaKeys;
+        const bool masked = lo > k0 || hi < k0 + kPaKeys;
+        if (__any_sync(0xffffffffu, masked)) {
+          // columns of the visible keys: up to the cut page as they are, in it behind the shift
+          const int lp = min(kPaKeys, last_page - k0);
+          const int a0 = lo - k0, a1 = min(hi - k0, shift ? lp : kPaKeys);
+          const int c0 = shift ? max(lp, lo - k0) + shift : kPaKeys, c1 = hi - k0 + shift;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            const bool see = (i >= a0 && i < a1) || (i >= c0 && i < c1);
+            if (!see) r[i] = 0xFF800000u;                         // -inf
+          }
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(r[i]));
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const bool rise = (mx - m) * a.c > kPaRise || (m == -INFINITY && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, rise)) {
+          const float alpha = rise ? pa_ex2((m - mx) * a.c) : 1.f;
+          if (rise) m = mx;
+          l *= alpha;
+          if (j > mine0) {                                        // o of the steps so far
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[32];
+              pa_ld32(o_col + 32 * q, o);
+              pa_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              pa_st32(o_col + 32 * q, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m * a.c;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float p0 = pa_ex2(fmaf(__uint_as_float(r[64 * q + 2 * i]), a.c, -base));
+            const float p1 = pa_ex2(fmaf(__uint_as_float(r[64 * q + 2 * i + 1]), a.c, -base));
+            sum[0] += p0;
+            sum[1] += p1;
+            p[i] = pa_pack(p0, p1);
+          }
+          pa_st32(s_col + 32 * q, p);
+        }
+        l += sum[0] + sum[1];
+        pa_wait_st();
+        pa_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_p[t]);
+      }
+      const bool any = mine0 < steps;
+      if (any && ok) {
+        if (!pa_wait(&b_o[t], (unsigned)o_par, &s_failed, status)) ok = false;
+        o_par ^= 1;
+        pa_fence_after();
+      }
+      if (!ok) break;
+      // two halves of one tile: group 1 hands its (m, l, o) over, 64 columns at a time
+      const bool join = !it.dual && steps > 1;
+      float f0 = 1.f, f1 = 0.f;
+      auto hand = [&](const uint32_t* o) {                        // group 1: 64 columns (and m, l beside the first ones)
+        if (handed > 0 && !pa_wait(&b_take, (unsigned)((handed - 1) & 1), &s_failed, status)) ok = false;
+        if ((handed & 1) == 0) s_ml[row] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sx[row * 16 + ((i + row) & 15)] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_hand);
+        ++handed;
+      };
+      auto take = [&](uint32_t* o) {                              // group 0
+        if (ok && !pa_wait(&b_hand, (unsigned)(handed & 1), &s_failed, status)) ok = false;
+        if ((handed & 1) == 0) {
+          const float2 other = s_ml[row];
+          const float mm = fmaxf(m, other.x);
+          f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c);
+          f1 = other.x == -INFINITY ? 0.f : pa_ex2((other.x - mm) * a.c);
+          l = l * f0 + other.y * f1;
+          m = mm;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float4 x = sx[row * 16 + ((i + row) & 15)];
+          o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * f0 + x.x * f1);
+          o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * f0 + x.y * f1);
+          o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * f0 + x.z * f1);
+          o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * f0 + x.w * f1);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b_take);
+        ++handed;
+      };
+      if (it.dual || t == 0 || join) {
+        const bool writes = valid && (it.dual || t == 0);
+        const int64_t slot_row = it.out >= 0 ? (int64_t)it.out * 256 + (it.dual ? t * 128 : 0) + row : 0;
+        const int64_t home_row = (int64_t)(it.home * a.batch + it.tok0 + tok) * a.Hkv * a.G + qh;
+        float inv = 1.f;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[64];
+          if (any) {
+            pa_ld32(o_col + 64 * half, o);
+            pa_ld32(o_col + 64 * half + 32, o + 32);
+            pa_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] = 0u;
+          }
+          if (join) {
+            if (t == 1) hand(o);
+            else take(o);
+          }
+          if (half == 0 && writes) {
+            if (it.out != PA_FINAL) *(it.out >= 0 ? a.ml + slot_row : a.home_ml + home_row) = make_float2(m, l);
+            else {
+              float den = l;
+              if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
+              inv = 1.0f / den;
+            }
+          }
+          if (!writes) continue;
+          if (it.out == PA_FINAL) {
+            bf16* dst = a.out + (int64_t)(it.tok0 + tok) * a.out_stride + qh * kPaD + 64 * half;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = m == -INFINITY ? 0u
+                                      : pa_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+              reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else if (m != -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                           __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              if (it.out >= 0) a.o[((int64_t)it.out * 32 + 16 * half + i) * 256 + (it.dual ? t * 128 : 0) + row] = x;
+              else a.home_o[home_row * 32 + 16 * half + i] = x;
+            }
+          }
+        }
+      }
+      pa_fence_before();                                          // o has been read: the next item's products may follow p
+    }
   }
+  pa_fence_before();
+  __syncthreads();
+  if (warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kPaTmem) : "memory");
+}
+
+// Joins the parts of the rows that were cut: a block per (token or stream, KV head), a thread per (head of the group, quad
+// of columns); the parts in the order of their keys, the prefix first.
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, int blocks) {
+  pdl_wait();
+  const int tok = blockIdx.x, h = blockIdx.y, g = threadIdx.x % a.G, quad = threadIdx.x / a.G;
+  const PaRecord own = a.rec[(int64_t)tok * a.Hkv + h];
+  if (own.first == 0 || own.first == PA_FINAL) return;
+  const int qh = h * a.G + g, per = kPaM / a.G;
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float2 ml, const float4* from) {
+    if (ml.x == -INFINITY) return;
+    const float4 x = *from;
+    const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c), f1 = pa_ex2((ml.x - mm) * a.c);
+    l = l * f0 + ml.y * f1;
+    o.x = o.x * f0 + x.x * f1, o.y = o.y * f0 + x.y * f1, o.z = o.z * f0 + x.z * f1, o.w = o.w * f0 + x.w * f1;
+    m = mm;
+  };
+  auto parts = [&](const PaRecord& r, int home) {
+    if (r.first == PA_HOME) {
+      const int64_t row = (int64_t)(home * a.batch + tok) * a.Hkv * a.G + qh;
+      add(a.home_ml[row], a.home_o + row * 32 + quad);
+      return;
+    }
+    const int at = tok - r.tok0, row = at / per * kPaM + at % per * a.G + g;
+    if (r.first < 1 || r.last > blocks || at < 0 || at >= 2 * per) return;
+#pragma unroll 4
+    for (int c = r.first; c <= r.last; ++c) {
+      const int64_t slot = 2 * (c - 1) + (c == r.first);
+      add(a.ml[slot * 256 + row], a.o + (slot * 32 + quad) * 256 + row);
+    }
+  };
+  if (!a.group_starts) {
+    __syncthreads();
+    if (threadIdx.x == 0) a.rec[(int64_t)tok * a.Hkv + h].first = 0;
+  }
+  if (own.prefix) parts(a.rec[((int64_t)a.batch + tok) * a.Hkv + h], 1);
+  parts(own, 0);
+  float den = l;
+  if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
+  const float inv = m == -INFINITY ? 0.f : 1.0f / den;
+  uint2 w = make_uint2(pa_pack(o.x * inv, o.y * inv), pa_pack(o.z * inv, o.w * inv));
+  reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.out_stride + qh * kPaD)[quad] = w;
 }
 
 }  // namespace flint
@@ -224,42 +885,78 @@ using namespace flint;
 
 int64_t flint::status_offset_paged_attention() { return (int64_t)offsetof(PagedAttnWorkspace, status); }
 
-static int paged_attn_check(const void* q, int64_t q_stride, const void* kv, int64_t num_blocks, int64_t Hkv,
-                            int64_t stride_block, int64_t stride_head, const int32_t* bt, int64_t bt_stride,
-                            int64_t max_blocks, const int32_t* seq_lens, int64_t window, int64_t batch, int64_t tokens,
-                            int64_t Hq, const void* out, int64_t out_stride, const void* ws) {
-  if (!q || !kv || !bt || !seq_lens || !out || !ws) return FLINT_ERR_ARGUMENT;
-  if (window < 0 || window > INT32_MAX) return FLINT_ERR_ARGUMENT;
-  if (batch < 1 || batch > 65535 || tokens < 1 || tokens > (1 << 24) || Hkv < 1 || Hkv > 128 || Hq < 1 || Hq % Hkv != 0 ||
-      Hq / Hkv > 8 || num_blocks < 1 || num_blocks > INT32_MAX || max_blocks < 1 || max_blocks > (1 << 26) ||
-      bt_stride < 0 || q_stride < Hq * kPaD || out_stride < Hq * kPaD || stride_head < kPaPage * 2 * kPaD ||
-      stride_block < stride_head)
-    return FLINT_ERR_SHAPE;
-  if (!aligned(kv, 16) || stride_block % 8 != 0 || stride_head % 8 != 0 || !aligned(out, 16) || !aligned(q, 16) ||
-      q_stride % 8 != 0 || out_stride % 8 != 0)
-    return FLINT_ERR_ALIGN;
-  if (num_sms() <= 0) return FLINT_ERR_DEVICE;
-  return FLINT_OK;
+// The workspace: status, then (m, l) and o of the slots (two per block), of a size that the device alone decides; behind
+// them a prompt's records, which the join clears, so that they are clear for calls of any shape; or, with shared prefixes,
+// the homes and the records, which every call writes before it reads them.
+struct PaLayout {
+  int64_t ml, o, rec, home_ml, home_o, bytes;
+};
+static PaLayout pa_layout(int64_t blocks, int64_t records, int64_t homes) {
+  PaLayout w;
+  w.ml = sizeof(PagedAttnWorkspace);
+  w.o = w.ml + blocks * 512 * (int64_t)sizeof(float2);
+  w.rec = w.o + blocks * 512 * 32 * (int64_t)sizeof(float4);
+  w.home_o = w.rec + (records * (int64_t)sizeof(PaRecord) + 127) / 128 * 128;
+  w.home_ml = w.home_o + homes * 32 * (int64_t)sizeof(float4);
+  w.bytes = w.home_ml + homes * (int64_t)sizeof(float2);
+  return w;
+}
+static int pa_blocks() {
+  const int n = num_sms();
+  return n > 0 ? n : 148;
 }
 
-static PagedAttnArgs paged_attn_args(const void* q, int64_t q_stride, const void* kv, int64_t num_blocks, int64_t Hkv,
-                                     int64_t stride_block, int64_t stride_head, const int32_t* bt, int64_t bt_stride,
-                                     int64_t max_blocks, const int32_t* seq_lens, const float* sinks, int64_t window,
-                                     float scale, int64_t batch, int64_t tokens, int64_t Hq, void* out,
-                                     int64_t out_stride, void* ws) {
+static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t num_blocks, int64_t Hkv, int64_t stride_block,
+                      int64_t stride_head, const int32_t* bt, int64_t bt_stride, int64_t max_blocks, const int32_t* cu_seqlens,
+                      const int32_t* seq_lens, const int32_t* group_starts, const int32_t* prefix_lens, int64_t groups,
+                      const float* sinks, int64_t window, float scale, int64_t batch, int64_t tokens, int64_t Hq, void* out,
+                      int64_t out_stride, void* ws, int pdl, void* stream) {
+  if (!q || !kv || !bt || !seq_lens || !out || !ws) return FLINT_ERR_ARGUMENT;
+  if (window < 0 || window > INT32_MAX || !(scale > 0.f) || !(scale < 1e30f)) return FLINT_ERR_ARGUMENT;
+  if (batch < 1 || batch > (1 << 20) || tokens < 1 || tokens > (1 << 24) || Hkv < 1 || Hkv > 128 || Hq < 1 || Hq % Hkv != 0 ||
+      Hq / Hkv > 8 || num_blocks < 1 || num_blocks >= INT32_MAX || max_blocks < 1 || max_blocks > (1 << 26) || bt_stride < 0 ||
+      q_stride < Hq * kPaD || out_stride < Hq * kPaD || stride_head < kPaPage * 2 * kPaD || stride_block < kPaPage * 2 * kPaD)
+    return FLINT_ERR_SHAPE;
+  if (!aligned(kv, 16) || stride_block % 8 != 0 || stride_head % 8 != 0 || !aligned(out, 16) || !aligned(q, 16) ||
+      q_stride % 8 != 0 || out_stride % 8 != 0 || !aligned(ws, 16))
+    return FLINT_ERR_ALIGN;
+  const int blocks = num_sms();
+  if (blocks <= 0) return FLINT_ERR_DEVICE;
+  const int G = (int)(Hq / Hkv), per = kPaM / G;
+  CUtensorMap mq, mkv;
+  const uint64_t qd[3] = {kPaD, (uint64_t)Hq, (uint64_t)tokens}, qs[2] = {kPaD * 2, (uint64_t)q_stride * 2};
+  const uint32_t qb[3] = {64, (uint32_t)G, (uint32_t)per};
+  int rc = encode_bf16_3d(&mq, q, qd, qs, qb);
+  if (rc) return rc;
+  const uint64_t kd[4] = {2 * kPaD, kPaPage, (uint64_t)Hkv, (uint64_t)num_blocks};
+  const uint64_t ks[3] = {2 * kPaD * 2, (uint64_t)stride_head * 2, (uint64_t)stride_block * 2};
+  const uint32_t kb[4] = {64, kPaPage, 1, 1};
+  rc = encode_bf16_4d(&mkv, kv, kd, ks, kb);
+  if (rc) return rc;
   PagedAttnArgs a = {};
-  a.q = (const bf16*)q; a.q_stride = q_stride; a.kv = (const bf16*)kv; a.stride_block = stride_block;
-  a.stride_head = stride_head; a.num_blocks = num_blocks; a.block_tables = bt; a.bt_stride = bt_stride;
-  a.max_blocks = (int)max_blocks; a.seq_lens = seq_lens; a.sinks = sinks; a.window = (int)window; a.batch = (int)batch;
-  a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = (int)(Hq / Hkv); a.c = scale * kPaLog2e; a.out = (bf16*)out;
-  a.out_stride = out_stride; a.ws = static_cast<PagedAttnWorkspace*>(ws);
-  return a;
+  a.block_tables = bt; a.bt_stride = bt_stride; a.max_blocks = (int)max_blocks; a.cu_seqlens = cu_seqlens;
+  a.seq_lens = seq_lens; a.group_starts = group_starts; a.prefix_lens = prefix_lens; a.groups = (int)groups; a.sinks = sinks;
+  a.window = (int)window; a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
+  a.num_blocks = (int)num_blocks; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
+  a.ws = static_cast<PagedAttnWorkspace*>(ws);
+  const PaLayout w = pa_layout(blocks, (group_starts ? 2 : 1) * tokens * Hkv, group_starts ? 2 * batch * Hq : 0);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  a.rec = reinterpret_cast<PaRecord*>(base + w.rec);
+  a.ml = reinterpret_cast<float2*>(base + w.ml);
+  a.o = reinterpret_cast<float4*>(base + w.o);
+  a.home_ml = reinterpret_cast<float2*>(base + w.home_ml);
+  a.home_o = reinterpret_cast<float4*>(base + w.home_o);
+  if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPaSmem) != cudaSuccess)
+    return FLINT_ERR_LAUNCH;
+  rc = launch(paged_attn_kernel, dim3((unsigned)blocks), dim3(kPaThreads), kPaSmem, stream, pdl, mq, mkv, a);
+  if (rc) return rc;
+  return launch(paged_join_kernel, dim3((unsigned)tokens, (unsigned)Hkv), dim3(32 * G), 0, stream, pdl, a, blocks);
 }
 
 extern "C" int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads,
                                                            int64_t num_kv_heads) {
   if (batch < 1 || tokens < 1 || num_q_heads < 1 || num_kv_heads < 1) return -1;
-  return (int64_t)sizeof(PagedAttnWorkspace);
+  return pa_layout(pa_blocks(), tokens * num_kv_heads, 0).bytes;
 }
 
 extern "C" int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_cache, int64_t num_blocks,
@@ -269,23 +966,15 @@ extern "C" int flint_prefill_attention(const void* q, int64_t q_stride_t, const 
                                        int64_t window, float scale, int64_t batch, int64_t tokens, int64_t num_q_heads,
                                        void* out, int64_t out_stride_t, void* workspace, int pdl, void* stream) {
   if (!cu_seqlens) return FLINT_ERR_ARGUMENT;
-  int rc = paged_attn_check(q, q_stride_t, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head, block_tables,
-                            bt_stride, max_blocks, seq_lens, window, batch, tokens, num_q_heads, out, out_stride_t,
-                            workspace);
-  if (rc) return rc;
-  PagedAttnArgs a = paged_attn_args(q, q_stride_t, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head,
-                                    block_tables, bt_stride, max_blocks, seq_lens, sinks, window, scale, batch, tokens,
-                                    num_q_heads, out, out_stride_t, workspace);
-  a.cu_seqlens = cu_seqlens;
-  const int tile_tokens = kPaRows / a.G;
-  const int64_t tiles = tokens / tile_tokens + batch;             // an upper bound of sum ceil(n_b / tile_tokens)
-  return launch(paged_attn_kernel, dim3((unsigned)tiles, (unsigned)num_kv_heads), dim3(128), 0, stream, pdl, a);
+  return paged_attn(q, q_stride_t, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head, block_tables, bt_stride,
+                    max_blocks, cu_seqlens, seq_lens, nullptr, nullptr, 0, sinks, window, scale, batch, tokens, num_q_heads,
+                    out, out_stride_t, workspace, pdl, stream);
 }
 
 extern "C" int64_t flint_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads,
                                                                  int64_t num_kv_heads) {
   if (batch < 1 || groups < 1 || num_q_heads < 1 || num_kv_heads < 1) return -1;
-  return (int64_t)sizeof(PagedAttnWorkspace);
+  return pa_layout(pa_blocks(), 2 * batch * num_kv_heads, 2 * batch * num_q_heads).bytes;
 }
 
 extern "C" int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, const void* kv_cache, int64_t num_blocks,
@@ -297,13 +986,7 @@ extern "C" int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, 
                                              int64_t out_stride_b, void* workspace, int pdl, void* stream) {
   if (!group_starts || !prefix_lens) return FLINT_ERR_ARGUMENT;
   if (groups < 1 || groups > batch) return FLINT_ERR_SHAPE;
-  int rc = paged_attn_check(q, q_stride_b, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head, block_tables,
-                            bt_stride, max_blocks, seq_lens, window, batch, batch, num_q_heads, out, out_stride_b,
-                            workspace);
-  if (rc) return rc;
-  PagedAttnArgs a = paged_attn_args(q, q_stride_b, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head,
-                                    block_tables, bt_stride, max_blocks, seq_lens, sinks, window, scale, batch, batch,
-                                    num_q_heads, out, out_stride_b, workspace);
-  a.group_starts = group_starts; a.prefix_lens = prefix_lens; a.groups = (int)groups;
-  return launch(paged_attn_kernel, dim3((unsigned)batch, (unsigned)num_kv_heads), dim3(128), 0, stream, pdl, a);
+  return paged_attn(q, q_stride_b, kv_cache, num_blocks, num_kv_heads, stride_block, stride_head, block_tables, bt_stride,
+                    max_blocks, nullptr, seq_lens, group_starts, prefix_lens, groups, sinks, window, scale, batch, batch,
+                    num_q_heads, out, out_stride_b, workspace, pdl, stream);
 }

@@ -189,6 +189,9 @@ int encode_u8_2d(CUtensorMap* map, const void* base, uint64_t cols_bytes, uint64
 // address A lands at unit u ^ ((A >> 7) & (swizzle_bytes / 16 - 1)).
 int encode_u8_2d_swz(CUtensorMap* map, const void* base, uint64_t cols_bytes, uint64_t rows, uint64_t row_stride_bytes,
                      uint32_t box_rows, int swizzle_bytes);
+// bf16 3-D map (dims innermost first, strides in bytes for dims 1..2), 128-byte swizzle.
+int encode_bf16_3d(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides_bytes[2],
+                   const uint32_t box[3]);
 // bf16 4-D map (dims innermost first, strides in bytes for dims 1..3), 128-byte swizzle.
 int encode_bf16_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides_bytes[3],
                    const uint32_t box[4]);

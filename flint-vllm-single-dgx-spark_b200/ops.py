@@ -871,7 +871,7 @@ def prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: tor
     _check_int32("prefill_attention", "cu_seqlens", cu_seqlens, B + 1, q.device)
     if T == 0 or B == 0:
         return
-    ws = _lib.workspace(q.device, "paged_attention", lib().flint_prefill_attention_workspace_bytes(B, T, Hq, Hkv))
+    ws = _lib.workspace(q.device, "prefill_attention", lib().flint_prefill_attention_workspace_bytes(B, T, Hq, Hkv))
     rc = lib().flint_prefill_attention(ptr(q), q.stride(0), ptr(kv_cache), nblk, Hkv, kv_cache.stride(0),
                                        kv_cache.stride(1), ptr(block_tables), block_tables.stride(0),
                                        block_tables.shape[1], ptr(cu_seqlens), ptr(seq_lens), ptr(sinks), int(window),
@@ -899,7 +899,8 @@ def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     _check_int32("shared_prefix_attention", "group_starts", group_starts, n + 1, q.device)
     if B == 0:
         return
-    ws = _lib.workspace(q.device, "paged_attention", lib().flint_shared_prefix_attention_workspace_bytes(B, n, Hq, Hkv))
+    ws = _lib.workspace(q.device, "shared_prefix_attention",
+                        lib().flint_shared_prefix_attention_workspace_bytes(B, n, Hq, Hkv))
     rc = lib().flint_shared_prefix_attention(ptr(q), q.stride(0), ptr(kv_cache), nblk, Hkv, kv_cache.stride(0),
                                              kv_cache.stride(1), ptr(block_tables), block_tables.stride(0),
                                              block_tables.shape[1], ptr(seq_lens), ptr(group_starts), ptr(prefix_lens),

@@ -251,6 +251,19 @@ def test_shared_long_suffixes(fb):
     run_shared(np.random.default_rng(14), [2, 1], [64, 0], [5000, 70, 3000], 2, 8, 0, False)
 
 
+def test_shared_many_short_suffixes(fb):
+    """Several items to a block, of one, two, three and more steps each, in every order."""
+    rng = np.random.default_rng(16)
+    lens = [64 + int(x) for x in rng.integers(0, 520, size=150)] + [int(x) for x in rng.integers(0, 400, size=90)]
+    run_shared(rng, [150, 90], [64, 0], lens, 8, 2, 0, True)
+
+
+def test_prefill_many_short_sequences(fb):
+    rng = np.random.default_rng(17)
+    q_lens = [int(x) for x in rng.integers(0, 40, size=60)]
+    run_prefill(rng, q_lens, [n + int(x) for n, x in zip(q_lens, rng.integers(0, 500, size=60))], 8, 4, 0, False)
+
+
 def test_shared_graph_replay(fb):
     from flint_b200 import shared_prefix_attention as sp
     args, out = run_shared(np.random.default_rng(15), [6, 2], [1024, 0], [1030, 1100, 0, 1025, 1200, 1024, 40, 7], 2, 8, 0,
