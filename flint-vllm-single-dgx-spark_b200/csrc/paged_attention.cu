@@ -26,6 +26,8 @@
 // its last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too.
 #include <limits.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "runtime.cuh"
 #include "tma.cuh"
@@ -946,8 +948,15 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   a.o = reinterpret_cast<float4*>(base + w.o);
   a.home_ml = reinterpret_cast<float2*>(base + w.home_ml);
   a.home_o = reinterpret_cast<float4*>(base + w.home_o);
-  if (cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPaSmem) != cudaSuccess)
-    return FLINT_ERR_LAUNCH;
+  static std::atomic<uint64_t> ready{0};                          // devices whose shared-memory limit is raised
+  int dev = 0;
+  num_sms(&dev);
+  if (!(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    rc = record_cuda(cudaFuncSetAttribute(paged_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPaSmem),
+                     FLINT_ERR_LAUNCH);
+    if (rc) return rc;
+    ready.fetch_or(uint64_t(1) << dev);
+  }
   rc = launch(paged_attn_kernel, dim3((unsigned)blocks), dim3(kPaThreads), kPaSmem, stream, pdl, mq, mkv, a);
   if (rc) return rc;
   return launch(paged_join_kernel, dim3((unsigned)tokens, (unsigned)Hkv), dim3(32 * G), 0, stream, pdl, a, blocks);

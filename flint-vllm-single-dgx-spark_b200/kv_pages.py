@@ -20,23 +20,23 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from . import ops as _ops  # noqa: F401  (registers torch.ops.flint_b200.*)
+from . import ops as _ops
 
 
 def flint_kv_reserve(ref, block_tables, seq_lens, num_pages, streams, lens):
-    torch.ops.flint_b200.kv_reserve(ref, block_tables, num_pages, streams, lens)
+    _ops.run("kv_reserve", ref, block_tables, num_pages, streams, lens)
 
 
 def flint_kv_fork(kv, ref, block_tables, seq_lens, num_pages, src, dst):
-    torch.ops.flint_b200.kv_fork(kv, ref, block_tables, seq_lens, num_pages, src, dst)
+    _ops.run("kv_fork", kv, ref, block_tables, seq_lens, num_pages, src, dst)
 
 
 def flint_kv_free(ref, block_tables, seq_lens, num_pages, streams):
-    torch.ops.flint_b200.kv_free(ref, block_tables, seq_lens, num_pages, streams)
+    _ops.run("kv_free", ref, block_tables, seq_lens, num_pages, streams)
 
 
 def flint_kv_compact(kv, ref, block_tables, num_pages, remap, live):
-    torch.ops.flint_b200.kv_compact(kv, ref, block_tables, num_pages, remap, live)
+    _ops.run("kv_compact", kv, ref, block_tables, num_pages, remap, live)
 
 
 class PagePool:

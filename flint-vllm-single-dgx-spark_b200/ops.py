@@ -829,55 +829,76 @@ def _(q, kv_cache, block_tables, seq_lens, sinks, window, scale, out, splits):
 # ------------------------------------------------------------------------------------------------------------
 # prompts and shared prompts over the paged cache
 # ------------------------------------------------------------------------------------------------------------
-def _check_paged(what, q, kv_cache, block_tables, seq_lens, sinks, out):
-    """Shapes and types that the prompt and shared-prefix attention have in common."""
+def run(name: str, *args) -> None:
+    """Op `name` of this section.  Its Python function is called directly, since the dispatcher's way to a Python kernel
+    takes more host time (20 of 40 us a call) than these launches; through torch.ops where a tracer or a dispatch mode
+    has to see the op."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        getattr(torch.ops.flint_b200, name)(*args)
+    else:
+        _DIRECT[name](*args)
+
+
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+
+
+def _check_paged(what, q, kv, bt, seq_lens, sinks, out):
+    """Shapes and types that the prompt and shared-prefix attention have in common -> the C ABI's arguments up to the
+    block tables, out's row stride.  (The stride of a dimension of one element says nothing and is not looked at.)"""
     _lib.require_cuda(q, what)
-    dev = q.device
-    if q.dim() != 3 or q.shape[2] != 128 or q.dtype != torch.bfloat16 or q.stride(2) != 1 or q.stride(1) != 128:
+    dev, shape, kv_shape, bt_shape = q.device, q.shape, kv.shape, bt.shape
+    qs, os, ks = q.stride(), out.stride(), kv.stride()
+    if len(shape) != 3 or shape[2] != 128 or q.dtype != _BF16 or qs[2] != 1 or (qs[1] != 128 and shape[1] != 1):
         raise _lib.FlintError(f"{what}: q must be bf16 [rows, heads, 128] with contiguous heads, got {q.dtype} "
-                              f"{tuple(q.shape)}")
-    if out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1 or out.stride(1) != 128:
-        raise _lib.FlintError(f"{what}: out must be bf16 {tuple(q.shape)} with contiguous heads")
-    if (kv_cache.dim() != 4 or kv_cache.shape[2] != 16 or kv_cache.shape[3] != 256 or kv_cache.dtype != torch.bfloat16
-            or kv_cache.stride(3) != 1 or kv_cache.stride(2) != 256):
+                              f"{tuple(shape)}")
+    T, Hq, _ = shape
+    if out.shape != shape or out.dtype != _BF16 or os[2] != 1 or (os[1] != 128 and Hq != 1):
+        raise _lib.FlintError(f"{what}: out must be bf16 {tuple(shape)} with contiguous heads")
+    if len(kv_shape) != 4 or kv_shape[2:] != (16, 256) or kv.dtype != _BF16 or ks[3] != 1 or ks[2] != 256:
         raise _lib.FlintError(f"{what}: kv_cache must be HND bf16 [blocks, kv_heads, 16, 256]")
-    if q.shape[1] % kv_cache.shape[1] or q.shape[1] > 8 * kv_cache.shape[1]:
-        raise _lib.FlintError(f"{what}: {q.shape[1]} query heads on {kv_cache.shape[1]} kv heads: 1 to 8 each")
-    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1
-            or seq_lens.dtype != torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous()
-            or block_tables.shape[0] < seq_lens.shape[0]):
+    nblk, Hkv, _, _ = kv_shape
+    if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= 8:
+        raise _lib.FlintError(f"{what}: {Hq} query heads on {Hkv} kv heads: 1 to 8 each")
+    if (bt.dtype != _I32 or seq_lens.dtype != _I32 or len(bt_shape) != 2 or seq_lens.dim() != 1
+            or (bt.stride(1) != 1 and bt_shape[1] != 1) or not seq_lens.is_contiguous() or bt_shape[0] < seq_lens.shape[0]):
         raise _lib.FlintError(f"{what}: block_tables must be int32 [batch, max_blocks] with rows contiguous, seq_lens "
                               "int32 [batch]")
-    if sinks is not None and (sinks.dtype != torch.float32 or sinks.numel() != q.shape[1] or not sinks.is_contiguous()):
-        raise _lib.FlintError(f"{what}: sinks must be fp32 [{q.shape[1]}]")
-    if (kv_cache.device != dev or block_tables.device != dev or seq_lens.device != dev or out.device != dev
-            or (sinks is not None and sinks.device != dev)):
+    if sinks is not None and (sinks.dtype != _F32 or sinks.numel() != Hq or not sinks.is_contiguous()
+                              or sinks.device != dev):
+        raise _lib.FlintError(f"{what}: sinks must be fp32 [{Hq}] on {dev}")
+    if kv.device != dev or bt.device != dev or seq_lens.device != dev or out.device != dev:
         raise _lib.FlintError(f"{what}: all tensors must be on {dev}")
+    row = Hq * 128
+    return ((q.data_ptr(), qs[0] if T > 1 else row, kv.data_ptr(), nblk, Hkv, ks[0] if nblk > 1 else Hkv * 4096,
+             ks[1] if Hkv > 1 else 4096, bt.data_ptr(), bt.stride(0) if bt_shape[0] > 1 else bt_shape[1], bt_shape[1]),
+            os[0] if T > 1 else row)
 
 
 def _check_int32(what, name, t, n, dev):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
+    if t.dtype != _I32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
         raise _lib.FlintError(f"{what}: {name} must be int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-@torch.library.custom_op(f"{NS}::prefill_attention", mutates_args=("out",))
-def prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
-                      seq_lens: torch.Tensor, sinks: torch.Tensor | None, window: int, scale: float,
-                      out: torch.Tensor) -> None:
+def _prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
+                       seq_lens: torch.Tensor, sinks: torch.Tensor | None, window: int, scale: float,
+                       out: torch.Tensor) -> None:
     """Causal attention of packed query tokens over the paged cache (flint_prefill_attention)."""
-    _check_paged("prefill_attention", q, kv_cache, block_tables, seq_lens, sinks, out)
-    T, Hq, B = q.shape[0], q.shape[1], seq_lens.shape[0]
-    nblk, Hkv = kv_cache.shape[0], kv_cache.shape[1]
-    _check_int32("prefill_attention", "cu_seqlens", cu_seqlens, B + 1, q.device)
+    args, out_stride = _check_paged("prefill_attention", q, kv_cache, block_tables, seq_lens, sinks, out)
+    T, Hq, _ = q.shape
+    B, dev = seq_lens.shape[0], q.device
+    _check_int32("prefill_attention", "cu_seqlens", cu_seqlens, B + 1, dev)
     if T == 0 or B == 0:
         return
-    ws = _lib.workspace(q.device, "prefill_attention", lib().flint_prefill_attention_workspace_bytes(B, T, Hq, Hkv))
-    rc = lib().flint_prefill_attention(ptr(q), q.stride(0), ptr(kv_cache), nblk, Hkv, kv_cache.stride(0),
-                                       kv_cache.stride(1), ptr(block_tables), block_tables.stride(0),
-                                       block_tables.shape[1], ptr(cu_seqlens), ptr(seq_lens), ptr(sinks), int(window),
-                                       float(scale), B, T, Hq, ptr(out), out.stride(0), ptr(ws), PDL,
-                                       stream_ptr(q.device))
-    check(rc, "flint_prefill_attention")
+    L = lib()
+    ws, stream = _lib.workspace_and_stream(dev, "prefill_attention",
+                                           L.flint_prefill_attention_workspace_bytes(B, T, Hq, args[4]))
+    rc = L.flint_prefill_attention(*args, cu_seqlens.data_ptr(), seq_lens.data_ptr(), ptr(sinks), window, scale, B, T, Hq,
+                                   out.data_ptr(), out_stride, ws, PDL, stream)
+    if rc:
+        check(rc, "flint_prefill_attention")
+
+
+prefill_attention = torch.library.custom_op(f"{NS}::prefill_attention", mutates_args=("out",))(_prefill_attention)
 
 
 @prefill_attention.register_fake
@@ -885,28 +906,30 @@ def _(q, kv_cache, block_tables, cu_seqlens, seq_lens, sinks, window, scale, out
     return None
 
 
-@torch.library.custom_op(f"{NS}::shared_prefix_attention", mutates_args=("out",))
-def shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
-                            group_starts: torch.Tensor, prefix_lens: torch.Tensor, sinks: torch.Tensor | None,
-                            window: int, scale: float, out: torch.Tensor) -> None:
+def _shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                             group_starts: torch.Tensor, prefix_lens: torch.Tensor, sinks: torch.Tensor | None,
+                             window: int, scale: float, out: torch.Tensor) -> None:
     """Decode attention of streams that share the first pages of their tables (flint_shared_prefix_attention)."""
-    _check_paged("shared_prefix_attention", q, kv_cache, block_tables, seq_lens, sinks, out)
-    B, Hq, n = q.shape[0], q.shape[1], prefix_lens.shape[0]
-    nblk, Hkv = kv_cache.shape[0], kv_cache.shape[1]
+    what = "shared_prefix_attention"
+    args, out_stride = _check_paged(what, q, kv_cache, block_tables, seq_lens, sinks, out)
+    B, Hq, _ = q.shape
+    n, dev = prefix_lens.numel(), q.device
     if seq_lens.shape[0] != B:
-        raise _lib.FlintError(f"shared_prefix_attention: {B} queries, {seq_lens.shape[0]} seq_lens")
-    _check_int32("shared_prefix_attention", "prefix_lens", prefix_lens, n, q.device)
-    _check_int32("shared_prefix_attention", "group_starts", group_starts, n + 1, q.device)
+        raise _lib.FlintError(f"{what}: {B} queries, {seq_lens.shape[0]} seq_lens")
+    _check_int32(what, "prefix_lens", prefix_lens, n, dev)
+    _check_int32(what, "group_starts", group_starts, n + 1, dev)
     if B == 0:
         return
-    ws = _lib.workspace(q.device, "shared_prefix_attention",
-                        lib().flint_shared_prefix_attention_workspace_bytes(B, n, Hq, Hkv))
-    rc = lib().flint_shared_prefix_attention(ptr(q), q.stride(0), ptr(kv_cache), nblk, Hkv, kv_cache.stride(0),
-                                             kv_cache.stride(1), ptr(block_tables), block_tables.stride(0),
-                                             block_tables.shape[1], ptr(seq_lens), ptr(group_starts), ptr(prefix_lens),
-                                             n, ptr(sinks), int(window), float(scale), B, Hq, ptr(out), out.stride(0),
-                                             ptr(ws), PDL, stream_ptr(q.device))
-    check(rc, "flint_shared_prefix_attention")
+    L = lib()
+    ws, stream = _lib.workspace_and_stream(dev, what, L.flint_shared_prefix_attention_workspace_bytes(B, n, Hq, args[4]))
+    rc = L.flint_shared_prefix_attention(*args, seq_lens.data_ptr(), group_starts.data_ptr(), prefix_lens.data_ptr(), n,
+                                         ptr(sinks), window, scale, B, Hq, out.data_ptr(), out_stride, ws, PDL, stream)
+    if rc:
+        check(rc, "flint_shared_prefix_attention")
+
+
+shared_prefix_attention = torch.library.custom_op(f"{NS}::shared_prefix_attention",
+                                                  mutates_args=("out",))(_shared_prefix_attention)
 
 
 @shared_prefix_attention.register_fake
@@ -917,42 +940,51 @@ def _(q, kv_cache, block_tables, seq_lens, group_starts, prefix_lens, sinks, win
 # ------------------------------------------------------------------------------------------------------------
 # pages of the cache
 # ------------------------------------------------------------------------------------------------------------
-def _check_pool(what, ref, block_tables, seq_lens, num_pages):
+def _check_pool(what, ref, bt, seq_lens, num_pages):
+    """-> the C ABI's arguments ref .. num_streams, and those of the workspace and stream."""
     _lib.require_cuda(ref, what)
-    _check_int32(what, "ref", ref, ref.numel(), ref.device)
-    S = num_pages.numel()
-    _check_int32(what, "num_pages", num_pages, S, ref.device)
+    dev, blocks, S, bt_shape = ref.device, ref.numel(), num_pages.numel(), bt.shape
+    _check_int32(what, "ref", ref, blocks, dev)
+    _check_int32(what, "num_pages", num_pages, S, dev)
+    if (bt.dtype != _I32 or len(bt_shape) != 2 or bt_shape[0] != S or (bt.stride(1) != 1 and bt_shape[1] != 1)
+            or bt.device != dev):
+        raise _lib.FlintError(f"{what}: block_tables must be int32 [{S}, max_blocks] with rows contiguous on {dev}")
+    args = (ref.data_ptr(), blocks, bt.data_ptr(), bt.stride(0) if S > 1 else bt_shape[1], bt_shape[1])
     if seq_lens is not None:
-        _check_int32(what, "seq_lens", seq_lens, S, ref.device)
-    if (block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != S
-            or block_tables.stride(1) != 1 or block_tables.device != ref.device):
-        raise _lib.FlintError(f"{what}: block_tables must be int32 [{S}, max_blocks] with rows contiguous on {ref.device}")
+        _check_int32(what, "seq_lens", seq_lens, S, dev)
+        args += (seq_lens.data_ptr(),)
+    return args + (num_pages.data_ptr(), S)
 
 
 def _check_kv(what, kv, ref):
-    if (kv.dim() != 5 or kv.shape[3] != 16 or kv.shape[4] != 256 or kv.dtype != torch.bfloat16 or kv.device != ref.device
-            or kv.shape[1] != ref.shape[0] or kv.stride(4) != 1 or kv.stride(3) != 256 or kv.stride(2) != 16 * 256):
-        raise _lib.FlintError(f"{what}: kv must be bf16 [layers, {ref.shape[0]}, kv_heads, 16, 256] with contiguous pages")
+    """-> the C ABI's arguments kv .. stride_block."""
+    shape, st = kv.shape, kv.stride()
+    if (len(shape) != 5 or shape[3:] != (16, 256) or kv.dtype != _BF16 or kv.device != ref.device
+            or shape[1] != ref.numel() or st[4] != 1 or st[3] != 256 or (st[2] != 4096 and shape[2] != 1)):
+        raise _lib.FlintError(f"{what}: kv must be bf16 [layers, {ref.numel()}, kv_heads, 16, 256] with contiguous pages")
+    page = shape[2] * 4096
+    return (kv.data_ptr(), shape[0], shape[2], st[0] if shape[0] > 1 else page * shape[1], st[1] if shape[1] > 1 else page)
 
 
-def _pages_ws(ref):
-    return ptr(_lib.workspace(ref.device, "kv_pages", lib().flint_kv_pages_workspace_bytes(ref.shape[0])))
+def _pages_ws(L, ref):
+    ws, stream = _lib.workspace_and_stream(ref.device, "kv_pages", L.flint_kv_pages_workspace_bytes(ref.numel()))
+    return ws, PDL, stream
 
 
-@torch.library.custom_op(f"{NS}::kv_reserve", mutates_args=("ref", "block_tables", "num_pages"))
-def kv_reserve(ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.Tensor, streams: torch.Tensor,
-               lens: torch.Tensor) -> None:
+def _kv_reserve(ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.Tensor, streams: torch.Tensor,
+                lens: torch.Tensor) -> None:
     """Pages for streams up to lens tokens (flint_kv_reserve)."""
-    _check_pool("kv_reserve", ref, block_tables, None, num_pages)
-    n = streams.numel()
+    pool, n, L = _check_pool("kv_reserve", ref, block_tables, None, num_pages), streams.numel(), lib()
     _check_int32("kv_reserve", "streams", streams, n, ref.device)
     _check_int32("kv_reserve", "lens", lens, n, ref.device)
     if n == 0:
         return
-    rc = lib().flint_kv_reserve(ptr(ref), ref.shape[0], ptr(block_tables), block_tables.stride(0), block_tables.shape[1],
-                                ptr(num_pages), num_pages.shape[0], ptr(streams), ptr(lens), n, _pages_ws(ref), PDL,
-                                stream_ptr(ref.device))
-    check(rc, "flint_kv_reserve")
+    rc = L.flint_kv_reserve(*pool, streams.data_ptr(), lens.data_ptr(), n, *_pages_ws(L, ref))
+    if rc:
+        check(rc, "flint_kv_reserve")
+
+
+kv_reserve = torch.library.custom_op(f"{NS}::kv_reserve", mutates_args=("ref", "block_tables", "num_pages"))(_kv_reserve)
 
 
 @kv_reserve.register_fake
@@ -960,22 +992,22 @@ def _(ref, block_tables, num_pages, streams, lens):
     return None
 
 
-@torch.library.custom_op(f"{NS}::kv_fork", mutates_args=("kv", "ref", "block_tables", "seq_lens", "num_pages"))
-def kv_fork(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
-            num_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+def _kv_fork(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+             num_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
     """Streams dst become copies of src, whole pages shared (flint_kv_fork)."""
-    _check_pool("kv_fork", ref, block_tables, seq_lens, num_pages)
-    _check_kv("kv_fork", kv, ref)
-    n = src.numel()
+    pool, n, L = _check_pool("kv_fork", ref, block_tables, seq_lens, num_pages), src.numel(), lib()
+    cache = _check_kv("kv_fork", kv, ref)
     _check_int32("kv_fork", "src", src, n, ref.device)
     _check_int32("kv_fork", "dst", dst, n, ref.device)
     if n == 0:
         return
-    rc = lib().flint_kv_fork(ptr(kv), kv.shape[0], kv.shape[2], kv.stride(0), kv.stride(1), ptr(ref), ref.shape[0],
-                             ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(seq_lens),
-                             ptr(num_pages), num_pages.shape[0], ptr(src), ptr(dst), n, _pages_ws(ref), PDL,
-                             stream_ptr(ref.device))
-    check(rc, "flint_kv_fork")
+    rc = L.flint_kv_fork(*cache, *pool, src.data_ptr(), dst.data_ptr(), n, *_pages_ws(L, ref))
+    if rc:
+        check(rc, "flint_kv_fork")
+
+
+kv_fork = torch.library.custom_op(f"{NS}::kv_fork",
+                                  mutates_args=("kv", "ref", "block_tables", "seq_lens", "num_pages"))(_kv_fork)
 
 
 @kv_fork.register_fake
@@ -983,19 +1015,20 @@ def _(kv, ref, block_tables, seq_lens, num_pages, src, dst):
     return None
 
 
-@torch.library.custom_op(f"{NS}::kv_free", mutates_args=("ref", "block_tables", "seq_lens", "num_pages"))
-def kv_free(ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, num_pages: torch.Tensor,
-            streams: torch.Tensor) -> None:
+def _kv_free(ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, num_pages: torch.Tensor,
+             streams: torch.Tensor) -> None:
     """Streams give their pages back (flint_kv_free)."""
-    _check_pool("kv_free", ref, block_tables, seq_lens, num_pages)
-    n = streams.numel()
+    pool, n, L = _check_pool("kv_free", ref, block_tables, seq_lens, num_pages), streams.numel(), lib()
     _check_int32("kv_free", "streams", streams, n, ref.device)
     if n == 0:
         return
-    rc = lib().flint_kv_free(ptr(ref), ref.shape[0], ptr(block_tables), block_tables.stride(0), block_tables.shape[1],
-                             ptr(seq_lens), ptr(num_pages), num_pages.shape[0], ptr(streams), n, _pages_ws(ref), PDL,
-                             stream_ptr(ref.device))
-    check(rc, "flint_kv_free")
+    rc = L.flint_kv_free(*pool, streams.data_ptr(), n, *_pages_ws(L, ref))
+    if rc:
+        check(rc, "flint_kv_free")
+
+
+kv_free = torch.library.custom_op(f"{NS}::kv_free",
+                                  mutates_args=("ref", "block_tables", "seq_lens", "num_pages"))(_kv_free)
 
 
 @kv_free.register_fake
@@ -1003,23 +1036,29 @@ def _(ref, block_tables, seq_lens, num_pages, streams):
     return None
 
 
-@torch.library.custom_op(f"{NS}::kv_compact", mutates_args=("kv", "ref", "block_tables", "remap", "live"))
-def kv_compact(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.Tensor,
-               remap: torch.Tensor, live: torch.Tensor) -> None:
+def _kv_compact(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.Tensor,
+                remap: torch.Tensor, live: torch.Tensor) -> None:
     """Used pages to the front of the pool (flint_kv_compact)."""
-    _check_pool("kv_compact", ref, block_tables, None, num_pages)
-    _check_kv("kv_compact", kv, ref)
-    _check_int32("kv_compact", "remap", remap, ref.shape[0], ref.device)
+    pool, L = _check_pool("kv_compact", ref, block_tables, None, num_pages), lib()
+    cache = _check_kv("kv_compact", kv, ref)
+    _check_int32("kv_compact", "remap", remap, ref.numel(), ref.device)
     _check_int32("kv_compact", "live", live, 1, ref.device)
-    rc = lib().flint_kv_compact(ptr(kv), kv.shape[0], kv.shape[2], kv.stride(0), kv.stride(1), ptr(ref), ref.shape[0],
-                                ptr(block_tables), block_tables.stride(0), block_tables.shape[1], ptr(num_pages),
-                                num_pages.shape[0], ptr(remap), ptr(live), _pages_ws(ref), PDL, stream_ptr(ref.device))
-    check(rc, "flint_kv_compact")
+    rc = L.flint_kv_compact(*cache, *pool, remap.data_ptr(), live.data_ptr(), *_pages_ws(L, ref))
+    if rc:
+        check(rc, "flint_kv_compact")
+
+
+kv_compact = torch.library.custom_op(f"{NS}::kv_compact",
+                                     mutates_args=("kv", "ref", "block_tables", "remap", "live"))(_kv_compact)
 
 
 @kv_compact.register_fake
 def _(kv, ref, block_tables, num_pages, remap, live):
     return None
+
+
+_DIRECT = dict(prefill_attention=_prefill_attention, shared_prefix_attention=_shared_prefix_attention,
+               kv_reserve=_kv_reserve, kv_fork=_kv_fork, kv_free=_kv_free, kv_compact=_kv_compact)
 
 
 # ------------------------------------------------------------------------------------------------------------

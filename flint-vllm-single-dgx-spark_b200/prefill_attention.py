@@ -12,12 +12,9 @@ CUDA-graph safe: the launch depends on the shapes only; lengths and tables are r
 """
 from __future__ import annotations
 
-import torch
-
-from . import ops as _ops  # noqa: F401  (registers torch.ops.flint_b200.*)
+from . import ops as _ops
 
 
 def flint_prefill_attention(q, kv_cache, block_tables, cu_seqlens, seq_lens, sinks, window, scale, out):
-    torch.ops.flint_b200.prefill_attention(q, kv_cache, block_tables, cu_seqlens, seq_lens, sinks, int(window or 0),
-                                           float(scale), out)
+    _ops.run("prefill_attention", q, kv_cache, block_tables, cu_seqlens, seq_lens, sinks, int(window or 0), float(scale), out)
     return out

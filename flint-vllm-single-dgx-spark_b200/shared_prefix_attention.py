@@ -9,13 +9,11 @@ CUDA-graph safe: the launch depends on the shapes only; lengths, groups and tabl
 """
 from __future__ import annotations
 
-import torch
-
-from . import ops as _ops  # noqa: F401  (registers torch.ops.flint_b200.*)
+from . import ops as _ops
 
 
 def flint_shared_prefix_attention(q, kv_cache, block_tables, seq_lens, group_starts, prefix_lens, sinks, window, scale,
                                   out):
-    torch.ops.flint_b200.shared_prefix_attention(q, kv_cache, block_tables, seq_lens, group_starts, prefix_lens, sinks,
-                                                 int(window or 0), float(scale), out)
+    _ops.run("shared_prefix_attention", q, kv_cache, block_tables, seq_lens, group_starts, prefix_lens, sinks,
+             int(window or 0), float(scale), out)
     return out
