@@ -27,10 +27,14 @@
 #include <limits.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "runtime.cuh"
+#include "timeline.cuh"
 #include "tma.cuh"
+
+FLINT_TL_BUFFER
 
 namespace flint {
 
@@ -46,11 +50,12 @@ constexpr int kPaQueue = 4;                    // items cut ahead
 constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA, items, one idle
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
+constexpr int kPaFmaPairs = 1;                 // of four pairs of exponentials, those done by the FMA pipes
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
 constexpr int kPaFixed = 160;                  // cost of an item beside its keys, in keys of one tile
 constexpr int kPaLeast = 256;                  // least share of a block, in keys of one tile
 constexpr unsigned STATUS_BAD_SEQ = 4u;
-constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 64 * 4;
+constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4 + 8 * 2048;
 
 struct PagedAttnWorkspace {
   unsigned status;
@@ -118,41 +123,70 @@ __device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void pa_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// The loads so far have come; r (32 registers of the last one) is named so that nothing that reads it moves ahead.
+__device__ __forceinline__ void pa_wait_ld(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// The whole MMA warp runs these, so that addresses and descriptors stay in uniform registers; one elected lane (the same
+// one every time) issues.  Inside a branch of one lane each MMA took some 125 cycles to issue, twice what it takes to run.
 __device__ __forceinline__ void pa_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+      : "memory");
 }
-// Shared-memory operand, 128-byte swizzle (rows of 128 B, 8 rows to 1,024 B).  K along the row: 8-row groups 1,024 B apart.
-// K down the rows (V): 8 rows of K 1,024 B apart, the next 64 columns `lead` bytes on.
-__device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lead) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+// Shared-memory operand, 128-byte swizzle (rows of 128 B, 8 rows to 1,024 B), as (low, high) words of its descriptor; the
+// low word counts 16-byte units and takes offsets.  K along the row: 8-row groups 1,024 B apart.  K down the rows (V):
+// 8 rows of K 1,024 B apart, the next 64 columns `lead` bytes on.
+__device__ __forceinline__ uint32_t pa_desc_lo(uint32_t addr, uint32_t lead) {
+  return ((addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
 }
+constexpr uint32_t kPaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // fp32 accumulator, bf16 operands, N = 128, M = 128
 constexpr uint32_t kPaIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 constexpr uint32_t kPaIdescPV = kPaIdescQK | (1u << 16);          // B with K down the rows
 __device__ __forceinline__ void pa_mma_qk(uint32_t d, uint32_t q, uint32_t k) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {                                   // 16 columns of Q and K at a time
-    const uint32_t off = (i >> 2) * kPaHalf + (i & 3) * 32;
+    const uint32_t off = ((i >> 2) * kPaHalf + (i & 3) * 32) >> 4;
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(pa_desc(q + off, 16)),
-        "l"(pa_desc(k + off, 16)), "r"(kPaIdescQK), "r"(i > 0 ? 1u : 0u)
+        "{\n.reg .pred p, e;\n.reg .b64 qd, kd;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %5, 0;\n"
+        "mov.b64 qd, {%1, %4};\nmov.b64 kd, {%2, %4};\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], qd, kd, %3, p;\n}" ::"r"(d), "r"(q + off), "r"(k + off),
+        "r"(kPaIdescQK), "r"(kPaDescHi), "r"(i > 0 ? 1u : 0u)
         : "memory");
   }
 }
-__device__ __forceinline__ void pa_mma_pv(uint32_t d, uint32_t p, uint32_t v, bool add) {
+// the last 96 keys, or the first 32; p: where P begins
+__device__ __forceinline__ void pa_mma_pv(uint32_t d, uint32_t p, uint32_t v, int part, bool add) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)                                     // 16 keys at a time: 8 columns of P, 16 rows of V
+  for (int i = part ? 0 : 2; i < (part ? 2 : 8); ++i) {           // 16 keys at a time: 8 columns of P, 16 rows of V
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(p + 8 * i),
-        "l"(pa_desc(v + i * 2048, kPaHalf)), "r"(kPaIdescPV), "r"(add || i > 0 ? 1u : 0u)
+        "{\n.reg .pred p, e;\n.reg .b64 vd;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %5, 0;\n"
+        "mov.b64 vd, {%2, %4};\n"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], vd, %3, p;\n}" ::"r"(d), "r"(p + 8 * i),
+        "r"(v + (uint32_t)((i * 2048) >> 4)), "r"(kPaIdescPV), "r"(kPaDescHi), "r"(add || part || i > 2 ? 1u : 0u)
         : "memory");
+  }
 }
 // TMA boxes without an L2 hint: other blocks read the same keys
 __device__ __forceinline__ void pa_tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
@@ -166,6 +200,53 @@ __device__ __forceinline__ void pa_tma_4d(uint32_t dst, const CUtensorMap* map, 
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
           "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
+}
+// pairs of fp32 in a 64-bit register
+__device__ __forceinline__ uint64_t pa_two(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 pa_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// bits lo .. hi - 1 of a word
+__device__ __forceinline__ uint32_t pa_bits(int lo, int hi) {
+  const uint32_t below_hi = hi >= 32 ? ~0u : hi > 0 ? (1u << hi) - 1 : 0u, below_lo = lo >= 32 ? ~0u : lo > 0 ? (1u << lo) - 1 : 0u;
+  return below_hi & ~below_lo;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two elements on the FMA pipes (the special-function unit gives 16 results a cycle and SM, fewer than a step of
+// two tiles needs to keep up with its products): x = n + f with n whole and |f| <= 1/2, from the rounding of the addition
+// of 1.5 * 2^23; 2^f by the polynomial of degree 3 with the least largest relative error on [-1/2, 1/2] (Remez exchange),
+// 7.5e-5, far below the 2^-8 of the rounding to bf16; n goes into the exponent.  Below 2^-120 it stays at 2^-120.
+__device__ __forceinline__ uint64_t pa_ex2_fma(uint64_t x2) {
+  float2 x = pa_split(x2);
+  x2 = pa_two(fmaxf(x.x, -120.f), fmaxf(x.y, -120.f));
+  const uint64_t t = pa_add2(x2, pa_two(12582912.f, 12582912.f));
+  const uint64_t f = pa_add2(x2, pa_fma2(t, pa_two(-1.f, -1.f), pa_two(12582912.f, 12582912.f)));
+  uint64_t p = pa_fma2(f, pa_two(0.05517167f, 0.05517167f), pa_two(0.24261113f, 0.24261113f));
+  p = pa_fma2(f, p, pa_two(0.69326097f, 0.69326097f));
+  p = pa_fma2(f, p, pa_two(0.99992806f, 0.99992806f));
+  const float2 n = pa_split(t), y = pa_split(p);
+  return pa_two(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
+                __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ float pa_ex2(float x) {
   float y;
@@ -205,10 +286,14 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile
 
 // ---- the items ----
 // sum over i < k of max(0, a + i * t)
-__device__ __forceinline__ long long pa_ramp(long long a, long long t, long long k) {
-  long long i0 = a < 0 ? (-a + t - 1) / t : 0;
+__device__ __forceinline__ long long pa_ramp(int a, int t, int k) {
+  int i0 = a < 0 ? (int)(((unsigned)-a + t - 1) / (unsigned)t) : 0;
   if (i0 > k) i0 = k;
-  return a * (k - i0) + t * ((k - 1) * k - (i0 - 1) * i0) / 2;
+  return (long long)a * (k - i0) + t * (((k - 1ll) * k - (i0 - 1ll) * i0) / 2);
+}
+// a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes some hundred cycles)
+__device__ __forceinline__ long long pa_div(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
 // A run of row tiles on one line: a prompt's, a group's (its prefix) or a stream's own keys.  Every field is the same for
@@ -283,22 +368,22 @@ struct PaLine {
   }
   __device__ int tokens_of(const PaSegment& s, int i) const { return min(tile, s.ntok - i * tile); }
   // keys that item i is taken to cost
-  __device__ long long keys(const PaSegment& s, int i) const {
+  __device__ int keys(const PaSegment& s, int i) const {
     if (s.home) return a.window > 0 ? min(s.hi, a.window) : s.hi;
-    const long long p = (long long)s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
-    return max(0ll, e) - max((long long)s.lo, b) > 0 ? max(0ll, e) - max((long long)s.lo, b) : 0;
+    const int p = s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
+    return max(0, max(0, e) - max(s.lo, b));
   }
-  __device__ long long weight(const PaSegment& s, int i) const { return (tokens_of(s, i) > per ? 2 : 1) * keys(s, i); }
+  __device__ long long weight(const PaSegment& s, int i) const { return (tokens_of(s, i) > per ? 2ll : 1ll) * keys(s, i); }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
     const int m = (s.ntok + tile - 1) / tile;
     if (k <= 0 || m == 0) return 0;
-    const long long whole = min(k, m - 1);     // the last item may be shorter
+    const int whole = min(k, m - 1);           // the last item may be shorter
     long long w;
-    if (s.home) w = 2 * whole * keys(s, 0);
+    if (s.home) w = 2ll * whole * keys(s, 0);
     else {
-      w = pa_ramp((long long)s.pos0 + tile, tile, whole);
-      if (a.window > 0) w -= pa_ramp((long long)s.pos0 - a.window + 1, tile, whole);
+      w = pa_ramp(s.pos0 + tile, tile, whole);
+      if (a.window > 0) w -= pa_ramp(s.pos0 - a.window + 1, tile, whole);
       w *= 2;
     }
     if (k >= m) w += weight(s, m - 1);
@@ -313,16 +398,17 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;                                             // two Q tiles, each two halves of 64 columns
   uint8_t* ring = sq + 2 * kPaSlotBytes;
-  float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 64 columns of o between the halves
+  float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 32 columns of o between the halves; stores
   __shared__ PaItem items[kPaQueue];
   __shared__ __align__(8) uint64_t b_item[kPaQueue], b_item_free[kPaQueue], b_full[kPaSlots], b_empty[kPaSlots], b_q, b_q_free,
-      b_s[2], b_p[2], b_o[2], b_hand, b_take;
+      b_s[2], b_p[4], b_o[2], b_hand, b_take;
   __shared__ float2 s_ml[kPaM];
   __shared__ uint32_t s_taddr;
   __shared__ int s_failed;                                        // a wait ran out: every warp leaves
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned* status = &a.ws->status;
   if (tid == 0) {
+    FLINT_TL(0);
     s_failed = 0;
     for (int i = 0; i < kPaQueue; ++i) {
       mbar_init(&b_item[i], 1);
@@ -338,7 +424,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     mbar_init(&b_take, 4);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b_s[t], 1);
-      mbar_init(&b_p[t], 4);
+      mbar_init(&b_p[2 * t], 4);                                  // P of the last 96 and of the first 32 keys
+      mbar_init(&b_p[2 * t + 1], 4);
       mbar_init(&b_o[t], 1);
     }
     fence_mbar_init();
@@ -353,25 +440,35 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   __syncthreads();
   pa_fence_after();
   const uint32_t tmem = s_taddr;
+  if (tid == 0) FLINT_TL(1);
+  if (tid == 256) {
+    tma_prefetch_desc(&mq);
+    tma_prefetch_desc(&mkv);
+  }
   pdl_wait();
   pdl_trigger();
+  if (tid == 0) FLINT_TL(2);
 
   if (warp == 10) {
     // ---- items: this block's share of the line ----
     const PaLine line(a);
     const int nseg = line.segments();
-    long long total = 0;
-    for (int i0 = 0; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
+    PaSegment mine = line.segment(lane);
+    long long total = mine.cost * a.Hkv;
+    for (int i0 = 32; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const long long shares = max(1ll, min((long long)gridDim.x, total / kPaLeast));
-    auto cut = [&](long long c) { return c >= shares ? total : total * c / shares; };
+    if (lane == 0) FLINT_TL(3);
+    // equal shares (of a sum over 32 bits' reach in 64): the first `rest` blocks have one unit more
+    const long long shares = max(1ll, min((long long)gridDim.x, pa_div(total, kPaLeast)));
+    const long long share = pa_div(total, shares), rest = total - share * shares;
+    auto cut = [&](long long c) { return c >= shares ? total : share * c + min(c, rest); };
     const long long x0 = cut(blockIdx.x), x1 = blockIdx.x < shares ? cut(blockIdx.x + 1) : x0;
     long long at = 0;                                             // cost of the segments before the chunk's lane 0
     int n_items = 0;
     bool ok = true;
     for (int i0 = 0; i0 < nseg && at < x1 && ok; i0 += 32) {
-      const PaSegment mine = line.segment(i0 + lane);
+      if (i0 > 0) mine = line.segment(i0 + lane);
       long long cum = mine.cost * a.Hkv;                          // inclusive scan over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -399,18 +496,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         const int m = (s.ntok + line.tile - 1) / line.tile;
         int h = 0, i = 0;
         if (x0 > seg0) {                                          // the first item that the share touches
-          h = (int)((x0 - seg0) / s.cost);
-          const long long y = (x0 - seg0) % s.cost;
-          int hi = m - 1;
-          while (i < hi) {
-            const int mid = (i + hi + 1) >> 1;
-            if (line.upto(s, mid) <= y) i = mid; else hi = mid - 1;
+          h = (int)pa_div(x0 - seg0, s.cost);
+          const long long y = x0 - seg0 - h * s.cost;
+          int hi = m;
+          while (hi - i > 1) {                                    // 32 places at a time
+            const int step = (hi - i + 31) / 32, k2 = i + lane * step;
+            const int below = __popc(__ballot_sync(0xffffffffu, k2 < hi && line.upto(s, k2) <= y));
+            i += (below - 1) * step;
+            hi = min(hi, i + step);
           }
         }
-        for (; h < a.Hkv && ok; ++h, i = 0)
-          for (; i < m; ++i) {
-            const long long start = seg0 + h * s.cost + line.upto(s, i), w = line.weight(s, i), stop = start + kPaFixed + w;
-            if (start >= x1) break;
+        long long start = seg0 + h * s.cost + line.upto(s, i), w = 0;
+        for (; h < a.Hkv && ok && start < x1; ++h, i = 0)
+          for (; i < m && start < x1; ++i, start += kPaFixed + w) {
+            w = line.weight(s, i);
+            const long long stop = start + kPaFixed + w;
             PaItem it;
             it.tok0 = s.tok0 + i * line.tile, it.ntok = line.tokens_of(s, i), it.h = h, it.table = s.table;
             it.dual = it.ntok > line.per;
@@ -434,11 +534,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
               if (it.begin > it.end) it.begin = it.end;
             }
             const int steps = (it.end - it.begin + kPaKeys - 1) / kPaKeys;
-            // which steps lie before place x of the line
+            // how many steps lie before place x of the line
+            const unsigned unit = steps ? max(1u, ((unsigned)w + steps - 1) / (unsigned)steps) : 1u;
             auto before = [&](long long x) -> int {
               if (x >= stop) return steps;
-              if (x <= start + kPaFixed || w <= 0) return 0;
-              return (int)min((long long)steps, (x - start - kPaFixed) * steps / w);
+              return x <= start + kPaFixed ? 0 : min(steps, (int)((unsigned)(x - start - kPaFixed) / unit));
             };
             it.j0 = before(x0), it.j1 = before(x1);
             PaRecord rec = {PA_NONE, PA_NONE, it.tok0, !s.home && s.lo > 0};
@@ -477,6 +577,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             if (lane == 0) {
               items[q] = it;
               mbar_arrive(&b_item[q]);
+              if (n_items == 0) FLINT_TL(4);
             }
             __syncwarp();
             ++n_items;
@@ -530,7 +631,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         }
         if (++slot == kPaSlots) slot = 0, parity ^= 1;
       };
-      load(it.j0, 0);
+      // Q as soon as its buffer is free; the keys need not wait for that
+      const bool early = mbar_try_wait(&b_q_free, (unsigned)((nq & 1) ^ 1));
+      if (!early) load(it.j0, 0);
       if (ok && !pa_wait(&b_q_free, (unsigned)((nq & 1) ^ 1), &s_failed, status)) ok = false;
       ++nq;
       if (ok && lane == 0) {
@@ -541,6 +644,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             pa_tma_3d(smem_u32(sq) + t * kPaSlotBytes + half * kPaHalf, &mq, half * 64, it.h * a.G, it.tok0 + t * per, &b_q);
       }
       __syncwarp();
+      if (early) load(it.j0, 0);
+      if (n == 0 && lane == 0) FLINT_TL(5);
       if (it.dual) {                                              // K0 V0 K1 V1 ..
         for (int j = it.j0; j < it.j1; ++j) {
           if (j > it.j0) load(j, 0);
@@ -556,95 +661,104 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     }
   } else if (warp == 9) {
     // ---- MMA ----
-    if (lane == 0) {
-      int slot = 0, parity = 0, p_par[2] = {0, 0}, nq = 0;
-      bool ok = true;
-      const uint32_t s_ring = smem_u32(ring), s_q = smem_u32(sq);
-      auto next = [&]() {                                         // the next slot of the ring, filled
-        const int at = slot;
-        if (ok && !pa_wait(&b_full[at], (unsigned)parity, &s_failed, status)) ok = false;
-        if (++slot == kPaSlots) slot = 0, parity ^= 1;
-        return at;
-      };
-      auto wait_p = [&](int t) {
-        if (ok && !pa_wait(&b_p[t], (unsigned)p_par[t], &s_failed, status)) ok = false;
-        p_par[t] ^= 1;
+    int slot = 0, parity = 0, p_par[2] = {0, 0}, nq = 0;
+    bool ok = true;
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t q_desc = pa_desc_lo(smem_u32(sq), 16), k_desc = pa_desc_lo(smem_u32(ring), 16),
+                   v_desc = pa_desc_lo(smem_u32(ring), kPaHalf);
+    constexpr uint32_t kTile = kPaSlotBytes >> 4;
+    auto next = [&]() {                                           // the next slot of the ring, filled
+      const int at = slot;
+      if (ok && !pa_wait(&b_full[at], (unsigned)parity, &s_failed, status)) ok = false;
+      if (++slot == kPaSlots) slot = 0, parity ^= 1;
+      return at;
+    };
+    auto qk = [&](int t, int q, int k) {                          // S of half t of the block
+      pa_mma_qk(base + 128 * t, q_desc + q * kTile, k_desc + k * kTile);
+      pa_commit(&b_s[t]);
+    };
+    auto pv = [&](int t, int v, bool add) {                       // O += P V, in two parts as P comes
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        if (ok && !pa_wait(&b_p[2 * t + part], (unsigned)p_par[t], &s_failed, status)) ok = false;
+        if (!ok) return;
         pa_fence_after();
-      };
-      for (int n = 0; ok; ++n) {
-        if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
-        const PaItem it = items[n % kPaQueue];
-        mbar_arrive(&b_item_free[n % kPaQueue]);
-        if (it.ntok == 0) break;
-        const int steps = it.j1 - it.j0;
-        if (steps == 0) continue;
-        if (!pa_wait(&b_q, (unsigned)(nq++ & 1), &s_failed, status)) break;
-        pa_fence_after();
-        if (it.dual) {
-          int k = next();
-          for (int t = 0; t < 2 && ok; ++t) {
-            pa_mma_qk(tmem + 128 * t, s_q + t * kPaSlotBytes, s_ring + k * kPaSlotBytes);
-            pa_commit(&b_s[t]);
+        pa_mma_pv(base + 256 + 128 * t, base + 128 * t + 64, v_desc + v * kTile, part, add);
+      }
+      p_par[t] ^= 1;
+    };
+    for (int n = 0; ok; ++n) {
+      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+      const PaItem& it = items[n % kPaQueue];
+      const int ntok = __shfl_sync(0xffffffffu, it.ntok, 0), dual = __shfl_sync(0xffffffffu, it.dual, 0),
+                steps = __shfl_sync(0xffffffffu, it.j1 - it.j0, 0);
+      if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
+      __syncwarp();
+      if (ntok == 0) break;
+      if (steps == 0) continue;
+      if (!pa_wait(&b_q, (unsigned)(nq++ & 1), &s_failed, status)) break;
+      if (n == 0 && lane == 0) FLINT_TL(6);
+      pa_fence_after();
+      if (dual) {
+        int k = next();
+        if (!ok) break;
+        qk(0, 0, k);
+        qk(1, 1, k);
+        pa_commit(&b_empty[k]);
+        if (steps == 1) pa_commit(&b_q_free);
+        for (int j = 0; j < steps && ok; ++j) {
+          const int v = next();
+          if (j + 1 < steps) k = next();
+          pv(0, v, j > 0);
+          if (!ok) break;
+          if (j + 1 < steps) {
+            qk(0, 0, k);
+          } else {
+            pa_commit(&b_o[0]);
           }
+          pv(1, v, j > 0);
+          if (!ok) break;
+          pa_commit(&b_empty[v]);
+          if (j + 1 < steps) {
+            qk(1, 1, k);
+            pa_commit(&b_empty[k]);
+            if (j + 2 == steps) pa_commit(&b_q_free);
+          } else {
+            pa_commit(&b_o[1]);
+          }
+        }
+      } else {
+        for (int t = 0; t < 2 && t < steps; ++t) {
+          const int k = next();
+          if (!ok) break;
+          qk(t, 0, k);
           pa_commit(&b_empty[k]);
-          if (steps == 1) pa_commit(&b_q_free);
-          for (int j = 0; j < steps && ok; ++j) {
-            const int v = next();
-            for (int t = 0; t < 2 && ok; ++t) {
-              wait_p(t);
-              if (!ok) break;
-              pa_mma_pv(tmem + 256 + 128 * t, tmem + 128 * t, s_ring + v * kPaSlotBytes, j > 0);
-              if (t == 1) pa_commit(&b_empty[v]);
-              if (j + 1 < steps) {
-                if (t == 0) k = next();
-                if (!ok) break;
-                pa_mma_qk(tmem + 128 * t, s_q + t * kPaSlotBytes, s_ring + k * kPaSlotBytes);
-                pa_commit(&b_s[t]);
-                if (t == 1) {
-                  pa_commit(&b_empty[k]);
-                  if (j + 2 == steps) pa_commit(&b_q_free);
-                }
-              } else {
-                pa_commit(&b_o[t]);
-              }
-            }
-          }
-        } else {
-          for (int t = 0; t < 2 && t < steps; ++t) {
+          if (t + 1 == steps) pa_commit(&b_q_free);
+        }
+        for (int j = 0; j < steps && ok; ++j) {
+          const int t = j & 1, v = next();
+          if (t) pv(1, v, j > 1);
+          else pv(0, v, j > 1);
+          if (!ok) break;
+          pa_commit(&b_empty[v]);
+          if (j + 2 < steps) {
             const int k = next();
             if (!ok) break;
-            pa_mma_qk(tmem + 128 * t, s_q, s_ring + k * kPaSlotBytes);
-            pa_commit(&b_s[t]);
+            qk(t, 0, k);
             pa_commit(&b_empty[k]);
-            if (t + 1 == steps) pa_commit(&b_q_free);
-          }
-          for (int j = 0; j < steps && ok; ++j) {
-            const int t = j & 1, v = next();
-            wait_p(t);
-            if (!ok) break;
-            pa_mma_pv(tmem + 256 + 128 * t, tmem + 128 * t, s_ring + v * kPaSlotBytes, j > 1);
-            pa_commit(&b_empty[v]);
-            if (j + 2 < steps) {
-              const int k = next();
-              if (!ok) break;
-              pa_mma_qk(tmem + 128 * t, s_q, s_ring + k * kPaSlotBytes);
-              pa_commit(&b_s[t]);
-              pa_commit(&b_empty[k]);
-              if (j + 3 == steps) pa_commit(&b_q_free);
-            } else {
-              pa_commit(&b_o[t]);
-            }
+            if (j + 3 == steps) pa_commit(&b_q_free);
+          } else {
+            pa_commit(&b_o[t]);
           }
         }
       }
     }
-    __syncwarp();
   } else if (warp < 8) {
     // ---- softmax: group t of 128 threads, one row each ----
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
-    int s_par = 0, o_par = 0, handed = 0;                         // handed: halves of o from group 1 to group 0 so far
+    int s_par = 0, o_par = 0, handed = 0;                         // handed: quarters of o from group 1 to group 0 so far
     bool ok = true;
     for (int n = 0; ok; ++n) {
       if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
@@ -674,26 +788,37 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         }
         s_par ^= 1;
         pa_fence_after();
-        uint32_t r[128];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) pa_ld32(s_col + 32 * q, r + 32 * q);
-        pa_wait_ld();
+        if (n == 0 && j == 0 && tid == 0) FLINT_TL(7);
         const int k0 = it.begin + (it.j0 + j) * kPaKeys;
-        const bool masked = lo > k0 || hi < k0 + kPaKeys;
-        if (__any_sync(0xffffffffu, masked)) {
-          // columns of the visible keys: up to the cut page as they are, in it behind the shift
+        const bool hidden = __any_sync(0xffffffffu, lo > k0 || hi < k0 + kPaKeys);
+        // a bit for each column whose key this row sees: up to the cut page as they are, in it behind the shift
+        uint32_t see[4];
+        if (hidden) {
           const int lp = min(kPaKeys, last_page - k0);
           const int a0 = lo - k0, a1 = min(hi - k0, shift ? lp : kPaKeys);
           const int c0 = shift ? max(lp, lo - k0) + shift : kPaKeys, c1 = hi - k0 + shift;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            const bool see = (i >= a0 && i < a1) || (i >= c0 && i < c1);
-            if (!see) r[i] = 0xFF800000u;                         // -inf
-          }
+          for (int q = 0; q < 4; ++q) see[q] = pa_bits(a0 - 32 * q, a1 - 32 * q) | pa_bits(c0 - 32 * q, c1 - 32 * q);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto hide = [&](uint32_t* r, int q) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(r[i]));
+          for (int i = 0; i < 32; ++i)
+            if (!(see[q] & (1u << i))) r[i] = 0xFF800000u;        // -inf
+        };
+        // First pass: the maximum, 32 columns at a time, the next ones on their way.  The scores are read again below: held
+        // for both passes they take 128 registers and leave too few for the exponentials to overlap.
+        uint32_t r[2][32];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        pa_ld32(s_col, r[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          pa_wait_ld(r[q & 1]);
+          if (q < 3) pa_ld32(s_col + 32 * (q + 1), r[(q + 1) & 1]);
+          if (hidden) hide(r[q & 1], q);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            top[(i >> 1) & 3] = pa_max3(top[(i >> 1) & 3], __uint_as_float(r[q & 1][i]), __uint_as_float(r[q & 1][i + 1]));
+        }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool rise = (mx - m) * a.c > kPaRise || (m == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, rise)) {
@@ -705,7 +830,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             for (int q = 0; q < 4; ++q) {
               uint32_t o[32];
               pa_ld32(o_col + 32 * q, o);
-              pa_wait_ld();
+              pa_wait_ld(o);
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
               pa_st32(o_col + 32 * q, o);
@@ -713,50 +838,73 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           }
         }
         const float base = m == -INFINITY ? 0.f : m * a.c;
-        float sum[2] = {0.f, 0.f};
+        const uint64_t c2 = pa_two(a.c, a.c), nb2 = pa_two(-base, -base);
+        uint64_t sum[2] = {0, 0};
+        // Second pass, from the last columns, which are still here, to the first: 32 keys' P take the 16 columns from
+        // 64 + 16 q on, whose scores have been read.
+        auto exps = [&](auto fma_too) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t p[32];
+          for (int q = 3; q >= 0; --q) {
+            uint32_t* x = r[q & 1];
+            if (q < 3) {
+              pa_wait_ld(x);
+              if (hidden) hide(x, q);
+            }
+            if (q > 0) pa_ld32(s_col + 32 * (q - 1), r[(q - 1) & 1]);
+            uint32_t p[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float p0 = pa_ex2(fmaf(__uint_as_float(r[64 * q + 2 * i]), a.c, -base));
-            const float p1 = pa_ex2(fmaf(__uint_as_float(r[64 * q + 2 * i + 1]), a.c, -base));
-            sum[0] += p0;
-            sum[1] += p1;
-            p[i] = pa_pack(p0, p1);
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t x2 = pa_fma2(pa_two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, nb2);
+              float2 e;
+              if (decltype(fma_too)::value && i % 4 < kPaFmaPairs) e = pa_split(pa_ex2_fma(x2));
+              else {
+                const float2 y = pa_split(x2);
+                e = make_float2(pa_ex2(y.x), pa_ex2(y.y));
+              }
+              sum[i & 1] = pa_add2(sum[i & 1], pa_two(e.x, e.y));
+              p[i] = pa_pack(e.x, e.y);
+            }
+            pa_st16(s_col + 64 + 16 * q, p);
+            if (q <= 1) {                                         // 96 keys: the MMA warp starts on them; then the rest
+              pa_wait_st();
+              pa_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&b_p[2 * t + 1 - q]);
+            }
           }
-          pa_st32(s_col + 32 * q, p);
-        }
-        l += sum[0] + sum[1];
-        pa_wait_st();
-        pa_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b_p[t]);
+        };
+        // hidden keys are -inf, which only the special-function unit turns into 0
+        if (hidden) exps(std::false_type{});
+        else exps(std::true_type{});
+        const float2 part = pa_split(pa_add2(sum[0], sum[1]));
+        l += part.x + part.y;
+        if (n == 0 && j == 0 && tid == 0) FLINT_TL(8);
       }
       const bool any = mine0 < steps;
       if (any && ok) {
         if (!pa_wait(&b_o[t], (unsigned)o_par, &s_failed, status)) ok = false;
         o_par ^= 1;
         pa_fence_after();
+        if (n == 0 && tid == 0) FLINT_TL(9);
       }
       if (!ok) break;
       // two halves of one tile: group 1 hands its (m, l, o) over, 64 columns at a time
       const bool join = !it.dual && steps > 1;
       float f0 = 1.f, f1 = 0.f;
-      auto hand = [&](const uint32_t* o) {                        // group 1: 64 columns (and m, l beside the first ones)
+      auto hand = [&](const uint32_t* o, int quarter) {           // group 1: 32 columns (and m, l beside the first ones)
         if (handed > 0 && !pa_wait(&b_take, (unsigned)((handed - 1) & 1), &s_failed, status)) ok = false;
-        if ((handed & 1) == 0) s_ml[row] = make_float2(m, l);
+        if (quarter == 0) s_ml[row] = make_float2(m, l);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          sx[row * 16 + ((i + row) & 15)] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+        for (int i = 0; i < 8; ++i)
+          sx[row * 8 + ((i + row) & 7)] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                      __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
         __syncwarp();
         if (lane == 0) mbar_arrive(&b_hand);
         ++handed;
       };
-      auto take = [&](uint32_t* o) {                              // group 0
+      auto take = [&](uint32_t* o, int quarter) {                 // group 0
         if (ok && !pa_wait(&b_hand, (unsigned)(handed & 1), &s_failed, status)) ok = false;
-        if ((handed & 1) == 0) {
+        if (quarter == 0) {
           const float2 other = s_ml[row];
           const float mm = fmaxf(m, other.x);
           f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c);
@@ -765,8 +913,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           m = mm;
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float4 x = sx[row * 16 + ((i + row) & 15)];
+        for (int i = 0; i < 8; ++i) {
+          const float4 x = sx[row * 8 + ((i + row) & 7)];
           o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * f0 + x.x * f1);
           o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * f0 + x.y * f1);
           o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * f0 + x.z * f1);
@@ -780,58 +928,80 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         const bool writes = valid && (it.dual || t == 0);
         const int64_t slot_row = it.out >= 0 ? (int64_t)it.out * 256 + (it.dual ? t * 128 : 0) + row : 0;
         const int64_t home_row = (int64_t)(it.home * a.batch + it.tok0 + tok) * a.Hkv * a.G + qh;
+        // Finished rows go out through shared memory, 32 columns of the warp's 32 rows at a time: lane k then writes 16 bytes
+        // of row 8 i + k / 4, so that a store covers 8 runs of 64 bytes and not 32 of 16.
+        uint4* stage = reinterpret_cast<uint4*>(sx + kPaM * 8) + warp * 128;
+        int64_t to[4];                                            // (-1: no such row)
+        if (it.out == PA_FINAL && (it.dual || t == 0)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 32 * (warp & 3) + 8 * i + (lane >> 2), tk = r / a.G + (it.dual ? t * per : 0);
+            to[i] = r / a.G < per && tk < it.ntok
+                        ? (int64_t)(it.tok0 + tk) * a.out_stride + (it.h * a.G + r % a.G) * kPaD + (lane & 3) * 8
+                        : -1;
+          }
+        }
         float inv = 1.f;
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t o[64];
+        for (int quarter = 0; quarter < 4; ++quarter) {
+          uint32_t o[32];
           if (any) {
-            pa_ld32(o_col + 64 * half, o);
-            pa_ld32(o_col + 64 * half + 32, o + 32);
-            pa_wait_ld();
+            pa_ld32(o_col + 32 * quarter, o);
+            pa_wait_ld(o);
           } else {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) o[i] = 0u;
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
           }
           if (join) {
-            if (t == 1) hand(o);
-            else take(o);
+            if (t == 1) hand(o, quarter);
+            else take(o, quarter);
           }
-          if (half == 0 && writes) {
-            if (it.out != PA_FINAL) *(it.out >= 0 ? a.ml + slot_row : a.home_ml + home_row) = make_float2(m, l);
-            else {
+          if (!it.dual && t == 1) continue;
+          if (quarter == 0) {
+            if (it.out != PA_FINAL) {
+              if (writes) *(it.out >= 0 ? a.ml + slot_row : a.home_ml + home_row) = make_float2(m, l);
+            } else {
               float den = l;
-              if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
+              if (a.sinks && valid && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
               inv = 1.0f / den;
             }
           }
-          if (!writes) continue;
           if (it.out == PA_FINAL) {
-            bf16* dst = a.out + (int64_t)(it.tok0 + tok) * a.out_stride + qh * kPaD + 64 * half;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 w[e] = m == -INFINITY ? 0u
                                       : pa_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-              reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              stage[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          } else if (m != -INFINITY) {
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 4; ++i) {
+              const int r = 8 * i + (lane >> 2);
+              const uint4 w = stage[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
+              if (to[i] >= 0) *reinterpret_cast<uint4*>(a.out + to[i] + 32 * quarter) = w;
+            }
+            __syncwarp();
+          } else if (writes && m != -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
               const float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                                            __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-              if (it.out >= 0) a.o[((int64_t)it.out * 32 + 16 * half + i) * 256 + (it.dual ? t * 128 : 0) + row] = x;
-              else a.home_o[home_row * 32 + 16 * half + i] = x;
+              if (it.out >= 0) a.o[((int64_t)it.out * 32 + 8 * quarter + i) * 256 + (it.dual ? t * 128 : 0) + row] = x;
+              else a.home_o[home_row * 32 + 8 * quarter + i] = x;
             }
           }
         }
       }
+      if (n == 0 && tid == 0) FLINT_TL(10);
       pa_fence_before();                                          // o has been read: the next item's products may follow p
     }
   }
   pa_fence_before();
   __syncthreads();
+  if (tid == 0) FLINT_TL(11);
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kPaTmem) : "memory");
 }
@@ -999,3 +1169,5 @@ extern "C" int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, 
                     max_blocks, nullptr, seq_lens, group_starts, prefix_lens, groups, sinks, window, scale, batch, batch,
                     num_q_heads, out, out_stride_b, workspace, pdl, stream);
 }
+
+FLINT_TL_READER(flint_timeline_paged_attention)
