@@ -27,7 +27,6 @@
 #include <limits.h>
 
 #include <atomic>
-#include <type_traits>
 
 #include "common.cuh"
 #include "runtime.cuh"
@@ -46,13 +45,13 @@ constexpr int kPaSlots = 4;                    // ring slots of 128 keys x 128 c
 constexpr int kPaSlotBytes = kPaKeys * kPaD * 2;
 constexpr int kPaHalf = kPaSlotBytes / 2;      // 64 columns
 constexpr int kPaPageHalf = kPaPage * 128;     // a page's 64 columns
+constexpr int kPaRuns = 2048;                  // runs of 32 segments whose costs are kept
 constexpr int kPaQueue = 4;                    // items cut ahead
 constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA, items, one idle
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
-constexpr int kPaFmaPairs = 1;                 // of four pairs of exponentials, those done by the FMA pipes
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaFixed = 160;                  // cost of an item beside its keys, in keys of one tile
+constexpr int kPaFixed2 = 560, kPaFixed1 = 300;  // cost of an item of two / one tiles beside its keys, in keys of one tile
 constexpr int kPaLeast = 256;                  // least share of a block, in keys of one tile
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4 + 8 * 2048;
@@ -130,6 +129,11 @@ __device__ __forceinline__ void pa_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void pa_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // The loads so far have come; r (32 registers of the last one) is named so that nothing that reads it moves ahead.
 __device__ __forceinline__ void pa_wait_ld(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -176,15 +180,15 @@ __device__ __forceinline__ void pa_mma_qk(uint32_t d, uint32_t q, uint32_t k) {
         : "memory");
   }
 }
-// the last 96 keys, or the first 32; p: where P begins
+// the last 112 keys, or the first 16; p: where P begins
 __device__ __forceinline__ void pa_mma_pv(uint32_t d, uint32_t p, uint32_t v, int part, bool add) {
 #pragma unroll
-  for (int i = part ? 0 : 2; i < (part ? 2 : 8); ++i) {           // 16 keys at a time: 8 columns of P, 16 rows of V
+  for (int i = part ? 0 : 1; i < (part ? 1 : 8); ++i) {           // 16 keys at a time: 8 columns of P, 16 rows of V
     asm volatile(
         "{\n.reg .pred p, e;\n.reg .b64 vd;\nelect.sync _|e, 0xffffffff;\nsetp.ne.b32 p, %5, 0;\n"
         "mov.b64 vd, {%2, %4};\n"
         "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], vd, %3, p;\n}" ::"r"(d), "r"(p + 8 * i),
-        "r"(v + (uint32_t)((i * 2048) >> 4)), "r"(kPaIdescPV), "r"(kPaDescHi), "r"(add || part || i > 2 ? 1u : 0u)
+        "r"(v + (uint32_t)((i * 2048) >> 4)), "r"(kPaIdescPV), "r"(kPaDescHi), "r"(add || part || i > 1 ? 1u : 0u)
         : "memory");
   }
 }
@@ -231,22 +235,6 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-// 2^x of two elements on the FMA pipes (the special-function unit gives 16 results a cycle and SM, fewer than a step of
-// two tiles needs to keep up with its products): x = n + f with n whole and |f| <= 1/2, from the rounding of the addition
-// of 1.5 * 2^23; 2^f by the polynomial of degree 3 with the least largest relative error on [-1/2, 1/2] (Remez exchange),
-// 7.5e-5, far below the 2^-8 of the rounding to bf16; n goes into the exponent.  Below 2^-120 it stays at 2^-120.
-__device__ __forceinline__ uint64_t pa_ex2_fma(uint64_t x2) {
-  float2 x = pa_split(x2);
-  x2 = pa_two(fmaxf(x.x, -120.f), fmaxf(x.y, -120.f));
-  const uint64_t t = pa_add2(x2, pa_two(12582912.f, 12582912.f));
-  const uint64_t f = pa_add2(x2, pa_fma2(t, pa_two(-1.f, -1.f), pa_two(12582912.f, 12582912.f)));
-  uint64_t p = pa_fma2(f, pa_two(0.05517167f, 0.05517167f), pa_two(0.24261113f, 0.24261113f));
-  p = pa_fma2(f, p, pa_two(0.69326097f, 0.69326097f));
-  p = pa_fma2(f, p, pa_two(0.99992806f, 0.99992806f));
-  const float2 n = pa_split(t), y = pa_split(p);
-  return pa_two(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
-                __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 __device__ __forceinline__ float pa_ex2(float x) {
   float y;
@@ -373,7 +361,9 @@ struct PaLine {
     const int p = s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
     return max(0, max(0, e) - max(s.lo, b));
   }
-  __device__ long long weight(const PaSegment& s, int i) const { return (tokens_of(s, i) > per ? 2ll : 1ll) * keys(s, i); }
+  __device__ bool dual(const PaSegment& s, int i) const { return tokens_of(s, i) > per; }
+  __device__ int fixed(const PaSegment& s, int i) const { return dual(s, i) ? kPaFixed2 : kPaFixed1; }
+  __device__ long long weight(const PaSegment& s, int i) const { return (dual(s, i) ? 2ll : 1ll) * keys(s, i); }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
     const int m = (s.ntok + tile - 1) / tile;
@@ -386,11 +376,11 @@ struct PaLine {
       if (a.window > 0) w -= pa_ramp(s.pos0 - a.window + 1, tile, whole);
       w *= 2;
     }
-    if (k >= m) w += weight(s, m - 1);
-    return w + (long long)kPaFixed * min(k, m);
+    if (k >= m) w += weight(s, m - 1) + fixed(s, m - 1);
+    return w + (long long)kPaFixed2 * whole;
   }
 };
-static_assert(kPaFixed > 0, "every item has a place on the line");
+static_assert(kPaFixed1 > 0 && kPaFixed2 > 0, "every item has a place on the line");
 
 __global__ void __launch_bounds__(kPaThreads, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const PagedAttnArgs a) {
@@ -424,7 +414,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     mbar_init(&b_take, 4);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b_s[t], 1);
-      mbar_init(&b_p[2 * t], 4);                                  // P of the last 96 and of the first 32 keys
+      mbar_init(&b_p[2 * t], 4);                                  // P of the last 112 and of the first 16 keys
       mbar_init(&b_p[2 * t + 1], 4);
       mbar_init(&b_o[t], 1);
     }
@@ -449,13 +439,29 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   pdl_trigger();
   if (tid == 0) FLINT_TL(2);
 
+  // what each run of 32 segments costs, by all warps; the ring is still empty
+  const PaLine line(a);
+  const int nseg = line.segments();
+  long long* runs = reinterpret_cast<long long*>(ring);
+  const int kept = (nseg + 31) / 32 <= kPaRuns ? (nseg + 31) / 32 : 0;
+  for (int i0 = 32 * warp; i0 < 32 * kept; i0 += kPaThreads) {
+    long long c = line.segment(i0 + lane).cost * a.Hkv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+    if (lane == 0) runs[i0 / 32] = c;
+  }
+  __syncthreads();
+  long long total = 0, my_run = 0;
+  if (warp == 10) {                                               // (read before the ring fills)
+    for (int i = lane; i < kept; i += 32) total += runs[i];
+    my_run = lane < kept ? runs[lane] : 0;
+  }
+  __syncthreads();
+
   if (warp == 10) {
     // ---- items: this block's share of the line ----
-    const PaLine line(a);
-    const int nseg = line.segments();
-    PaSegment mine = line.segment(lane);
-    long long total = mine.cost * a.Hkv;
-    for (int i0 = 32; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
+    if (!kept)
+      for (int i0 = 0; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     if (lane == 0) FLINT_TL(3);
@@ -468,7 +474,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     int n_items = 0;
     bool ok = true;
     for (int i0 = 0; i0 < nseg && at < x1 && ok; i0 += 32) {
-      if (i0 > 0) mine = line.segment(i0 + lane);
+      if (kept && i0 < 32 * 32) {                                 // a run before the share
+        const long long c = __shfl_sync(0xffffffffu, my_run, i0 / 32);
+        if (at + c <= x0) {
+          at += c;
+          continue;
+        }
+      }
+      const PaSegment mine = line.segment(i0 + lane);
       long long cum = mine.cost * a.Hkv;                          // inclusive scan over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -507,10 +520,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           }
         }
         long long start = seg0 + h * s.cost + line.upto(s, i), w = 0;
+        int fixed = 0;
         for (; h < a.Hkv && ok && start < x1; ++h, i = 0)
-          for (; i < m && start < x1; ++i, start += kPaFixed + w) {
-            w = line.weight(s, i);
-            const long long stop = start + kPaFixed + w;
+          for (; i < m && start < x1; ++i, start += fixed + w) {
+            w = line.weight(s, i), fixed = line.fixed(s, i);
+            const long long stop = start + fixed + w;
             PaItem it;
             it.tok0 = s.tok0 + i * line.tile, it.ntok = line.tokens_of(s, i), it.h = h, it.table = s.table;
             it.dual = it.ntok > line.per;
@@ -538,7 +552,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             const unsigned unit = steps ? max(1u, ((unsigned)w + steps - 1) / (unsigned)steps) : 1u;
             auto before = [&](long long x) -> int {
               if (x >= stop) return steps;
-              return x <= start + kPaFixed ? 0 : min(steps, (int)((unsigned)(x - start - kPaFixed) / unit));
+              return x <= start + fixed ? 0 : min(steps, (int)((unsigned)(x - start - fixed) / unit));
             };
             it.j0 = before(x0), it.j1 = before(x1);
             PaRecord rec = {PA_NONE, PA_NONE, it.tok0, !s.home && s.lo > 0};
@@ -777,6 +791,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         if (a.window > 0) lo = max(0, hi - a.window);
         hi = max(0, min(hi, it.end));
       }
+      const bool idle = !__any_sync(0xffffffffu, valid);
       float m = -INFINITY, l = 0.f;
       const int stride = it.dual ? 1 : 2, mine0 = it.dual ? 0 : t;
       const int last_page = it.end & ~(kPaPage - 1);              // a cut last page: its tokens lie at its slot's end
@@ -789,6 +804,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         s_par ^= 1;
         pa_fence_after();
         if (n == 0 && j == 0 && tid == 0) FLINT_TL(7);
+        if (idle) {                                               // no row of this warp is one: P may be anything
+          pa_fence_before();
+          if (lane == 0) {
+            mbar_arrive(&b_p[2 * t]);
+            mbar_arrive(&b_p[2 * t + 1]);
+          }
+          continue;
+        }
         const int k0 = it.begin + (it.j0 + j) * kPaKeys;
         const bool hidden = __any_sync(0xffffffffu, lo > k0 || hi < k0 + kPaKeys);
         // a bit for each column whose key this row sees: up to the cut page as they are, in it behind the shift
@@ -805,19 +828,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           for (int i = 0; i < 32; ++i)
             if (!(see[q] & (1u << i))) r[i] = 0xFF800000u;        // -inf
         };
-        // First pass: the maximum, 32 columns at a time, the next ones on their way.  The scores are read again below: held
-        // for both passes they take 128 registers and leave too few for the exponentials to overlap.
-        uint32_t r[2][32];
+        // First pass: the maximum.  The first 64 columns are read again below: all 128 held for both passes leave too few
+        // registers for the exponentials to overlap.
+        uint32_t r[4][32];
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        pa_ld32(s_col, r[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pa_ld32(s_col + 32 * q, r[q]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          pa_wait_ld(r[q & 1]);
-          if (q < 3) pa_ld32(s_col + 32 * (q + 1), r[(q + 1) & 1]);
-          if (hidden) hide(r[q & 1], q);
+          pa_wait_ld(r[q]);
+          if (hidden) hide(r[q], q);
 #pragma unroll
           for (int i = 0; i < 32; i += 2)
-            top[(i >> 1) & 3] = pa_max3(top[(i >> 1) & 3], __uint_as_float(r[q & 1][i]), __uint_as_float(r[q & 1][i + 1]));
+            top[(i >> 1) & 3] = pa_max3(top[(i >> 1) & 3], __uint_as_float(r[q][i]), __uint_as_float(r[q][i + 1]));
         }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         const bool rise = (mx - m) * a.c > kPaRise || (m == -INFINITY && mx > -INFINITY);
@@ -842,40 +865,39 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         uint64_t sum[2] = {0, 0};
         // Second pass, from the last columns, which are still here, to the first: 32 keys' P take the 16 columns from
         // 64 + 16 q on, whose scores have been read.
-        auto exps = [&](auto fma_too) {
 #pragma unroll
-          for (int q = 3; q >= 0; --q) {
-            uint32_t* x = r[q & 1];
-            if (q < 3) {
-              pa_wait_ld(x);
-              if (hidden) hide(x, q);
-            }
-            if (q > 0) pa_ld32(s_col + 32 * (q - 1), r[(q - 1) & 1]);
-            uint32_t p[16];
+        for (int q = 3; q >= 0; --q) {
+          uint32_t* x = r[q];
+          if (q == 1) {
+            pa_wait_ld(r[1]);
+            pa_wait_ld(r[0]);
+            if (hidden) hide(r[1], 1), hide(r[0], 0);
+          }
+          if (q == 2) pa_ld32(s_col + 32, r[1]), pa_ld32(s_col, r[0]);
+          uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const uint64_t x2 = pa_fma2(pa_two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, nb2);
-              float2 e;
-              if (decltype(fma_too)::value && i % 4 < kPaFmaPairs) e = pa_split(pa_ex2_fma(x2));
-              else {
-                const float2 y = pa_split(x2);
-                e = make_float2(pa_ex2(y.x), pa_ex2(y.y));
-              }
-              sum[i & 1] = pa_add2(sum[i & 1], pa_two(e.x, e.y));
-              p[i] = pa_pack(e.x, e.y);
-            }
-            pa_st16(s_col + 64 + 16 * q, p);
-            if (q <= 1) {                                         // 96 keys: the MMA warp starts on them; then the rest
+          for (int i = 15; i >= 0; --i) {
+            const float2 y = pa_split(pa_fma2(pa_two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, nb2));
+            const float p0 = pa_ex2(y.x), p1 = pa_ex2(y.y);
+            sum[i & 1] = pa_add2(sum[i & 1], pa_two(p0, p1));
+            p[i] = pa_pack(p0, p1);
+            if (q == 0 && i == 8) {                               // all but the first 16 keys: the MMA warp starts on them
+              pa_st8(s_col + 64 + 8, p + 8);
               pa_wait_st();
               pa_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&b_p[2 * t + 1 - q]);
+              if (lane == 0) mbar_arrive(&b_p[2 * t]);
             }
           }
-        };
-        // hidden keys are -inf, which only the special-function unit turns into 0
-        if (hidden) exps(std::false_type{});
-        else exps(std::true_type{});
+          if (q > 0) pa_st16(s_col + 64 + 16 * q, p);
+          else {
+            pa_st8(s_col + 64, p);
+            pa_wait_st();
+            pa_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_p[2 * t + 1]);
+          }
+        }
         const float2 part = pa_split(pa_add2(sum[0], sum[1]));
         l += part.x + part.y;
         if (n == 0 && j == 0 && tid == 0) FLINT_TL(8);
