@@ -189,8 +189,10 @@ class FlintModel:
         # paged KV cache: FlashInfer HND [blocks, kv_heads, 16, 2*D] per layer; each stream owns a shuffled block set
         self.blocks_per_stream = (max_ctx + PAGE - 1) // PAGE
         nblk = self.blocks_per_stream * max_batch
-        self.kv = [torch.zeros((nblk, c.num_kv_heads, PAGE, 2 * c.head_dim), dtype=torch.bfloat16, device=self.dev)
-                   for _ in range(c.layers)]
+        # (one tensor of all layers, so that a page operation reaches a page's every layer)
+        self.kv_all = torch.zeros((c.layers, nblk, c.num_kv_heads, PAGE, 2 * c.head_dim), dtype=torch.bfloat16,
+                                  device=self.dev)
+        self.kv = list(self.kv_all)
         perm = torch.randperm(nblk, generator=torch.Generator().manual_seed(seed + 1)).to(torch.int32)
         self.block_tables = perm.reshape(max_batch, self.blocks_per_stream).to(self.dev).contiguous()
 
