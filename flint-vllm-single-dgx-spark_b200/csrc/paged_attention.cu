@@ -51,8 +51,9 @@ constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA,
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaFixed2 = 560, kPaFixed1 = 300;  // cost of an item of two / one tiles beside its keys, in keys of one tile
-constexpr int kPaLeast = 256;                  // least share of a block, in keys of one tile
+constexpr int kPaKey2 = 4, kPaKey1 = 3;        // cost of a key of an item of two / one tiles: 128 keys take 2.0 / 1.5 us,
+constexpr int kPaFixed2 = 1100, kPaFixed1 = 700;  // and of an item beside its keys: 4.3 / 2.7 us
+constexpr int kPaLeast = 800;                  // least share of a block
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4 + 8 * 2048;
 
@@ -61,14 +62,16 @@ struct PagedAttnWorkspace {
   unsigned pad[31];
 };
 
-// Where the parts of a token's result are: with blocks first .. last (counted from 1), or one of the values below in
-// `first`.  0 in `first`: nothing to join, what the join leaves behind for prompts (whose spare rows have no item).
-struct PaRecord {
+// Where the parts of an item are: with blocks first .. last, or one of the values below in `first`.
+enum { PA_FINAL = -1, PA_HOME = -2, PA_NONE = -3 };
+struct PaSplit {                               // a prompt's item that a block began and did not end
+  int first, last, tok0, ntok, h;
+};
+struct PaRecord {                              // a stream's own keys, or its group's prefix, for one KV head
   int first, last;
-  int tok0;                                    // the item's first token
+  int tok0;                                    // the item's first stream
   int prefix;                                  // of a stream's own keys: its group's prefix has a record too
 };
-enum { PA_FINAL = -1, PA_HOME = -2, PA_NONE = -3 };
 
 struct PagedAttnArgs {
   int64_t bt_stride;
@@ -84,7 +87,8 @@ struct PagedAttnArgs {
   bf16* out;
   int64_t out_stride;
   PagedAttnWorkspace* ws;
-  PaRecord* rec;                               // [tokens][Hkv] (shared: own keys, then [batch][Hkv] prefixes)
+  PaSplit* split;                              // prompts: one for each block (ntok 0: none)
+  PaRecord* rec;                               // shared prefixes: [batch][Hkv] own keys, then [batch][Hkv] prefixes
   float2 *ml, *home_ml;                        // (m, l): slots [2 x blocks][256 rows], homes [2][batch][Hq]
   float4 *o, *home_o;                          // the same rows' o: slots [32 quads of columns][256 rows], homes [row][32]
 };
@@ -363,19 +367,19 @@ struct PaLine {
   }
   __device__ bool dual(const PaSegment& s, int i) const { return tokens_of(s, i) > per; }
   __device__ int fixed(const PaSegment& s, int i) const { return dual(s, i) ? kPaFixed2 : kPaFixed1; }
-  __device__ long long weight(const PaSegment& s, int i) const { return (dual(s, i) ? 2ll : 1ll) * keys(s, i); }
+  __device__ long long weight(const PaSegment& s, int i) const { return (dual(s, i) ? (long long)kPaKey2 : kPaKey1) * keys(s, i); }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
     const int m = (s.ntok + tile - 1) / tile;
     if (k <= 0 || m == 0) return 0;
     const int whole = min(k, m - 1);           // the last item may be shorter
     long long w;
-    if (s.home) w = 2ll * whole * keys(s, 0);
+    if (s.home) w = (long long)whole * keys(s, 0);
     else {
       w = pa_ramp(s.pos0 + tile, tile, whole);
       if (a.window > 0) w -= pa_ramp(s.pos0 - a.window + 1, tile, whole);
-      w *= 2;
     }
+    w *= kPaKey2;
     if (k >= m) w += weight(s, m - 1) + fixed(s, m - 1);
     return w + (long long)kPaFixed2 * whole;
   }
@@ -473,6 +477,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     long long at = 0;                                             // cost of the segments before the chunk's lane 0
     int n_items = 0;
     bool ok = true;
+    PaSplit cut_item = {};
     for (int i0 = 0; i0 < nseg && at < x1 && ok; i0 += 32) {
       if (kept && i0 < 32 * 32) {                                 // a run before the share
         const long long c = __shfl_sync(0xffffffffu, my_run, i0 / 32);
@@ -571,17 +576,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
                 rec.first = it.out;
               } else {
                 it.out = 2 * blockIdx.x + (it.j0 == 0);
-                rec.first = blockIdx.x + 1;
+                rec.first = blockIdx.x;
                 if (first) {
                   long long c = blockIdx.x + 1;
                   while (before(cut(c)) < steps) ++c;
-                  rec.last = (int)c;
+                  rec.last = (int)c - 1;
                 }
               }
             }
-            if (first) {
+            if (first && line.shared) {
               PaRecord* to = a.rec + (s.home ? (int64_t)a.batch * a.Hkv : 0);
               for (int r = lane; r < it.ntok; r += 32) to[(int64_t)(it.tok0 + r) * a.Hkv + h] = rec;
+            } else if (first && rec.first >= 0) {
+              cut_item = {rec.first, rec.last, it.tok0, it.ntok, h};
             }
             const int q = n_items % kPaQueue;
             if (n_items >= kPaQueue && !pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status)) {
@@ -599,6 +606,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       }
       at += chunk;
     }
+    if (lane == 0 && !line.shared) a.split[blockIdx.x] = cut_item;
     // an item without tokens ends the block
     const int q = n_items % kPaQueue;
     if (n_items >= kPaQueue && ok) ok = pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status);
@@ -1028,49 +1036,79 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kPaTmem) : "memory");
 }
 
-// Joins the parts of the rows that were cut: a block per (token or stream, KV head), a thread per (head of the group, quad
-// of columns); the parts in the order of their keys, the prefix first.
+// Joins the parts of the rows that were cut: 8 rows at a time, a thread per row and quad of columns.  Prompts: kPaJoin
+// blocks for each item that was cut; streams: a block for 8 of their rows.  Parts are added in the order of their keys, the
+// prefix first; their (m, l), then their o, are loaded eight at a time, since what this costs is the latency of L2.
+constexpr int kPaJoin = 4;
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, int blocks) {
   pdl_wait();
-  const int tok = blockIdx.x, h = blockIdx.y, g = threadIdx.x % a.G, quad = threadIdx.x / a.G;
-  const PaRecord own = a.rec[(int64_t)tok * a.Hkv + h];
-  if (own.first == 0 || own.first == PA_FINAL) return;
-  const int qh = h * a.G + g, per = kPaM / a.G;
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, const float4* from) {
+  const int sub = threadIdx.x & 7, quad = threadIdx.x >> 3, per = kPaM / a.G;
+  float m, l;
+  float4 o;
+  auto add = [&](float2 ml, float4 x) {
     if (ml.x == -INFINITY) return;
-    const float4 x = *from;
     const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c), f1 = pa_ex2((ml.x - mm) * a.c);
     l = l * f0 + ml.y * f1;
     o.x = o.x * f0 + x.x * f1, o.y = o.y * f0 + x.y * f1, o.z = o.z * f0 + x.z * f1, o.w = o.w * f0 + x.w * f1;
     m = mm;
   };
-  auto parts = [&](const PaRecord& r, int home) {
-    if (r.first == PA_HOME) {
-      const int64_t row = (int64_t)(home * a.batch + tok) * a.Hkv * a.G + qh;
-      add(a.home_ml[row], a.home_o + row * 32 + quad);
-      return;
-    }
-    const int at = tok - r.tok0, row = at / per * kPaM + at % per * a.G + g;
-    if (r.first < 1 || r.last > blocks || at < 0 || at >= 2 * per) return;
-#pragma unroll 4
-    for (int c = r.first; c <= r.last; ++c) {
-      const int64_t slot = 2 * (c - 1) + (c == r.first);
-      add(a.ml[slot * 256 + row], a.o + (slot * 32 + quad) * 256 + row);
+  auto parts = [&](int first, int last, int at, int g) {          // at: the token's place in its item
+    const int row = at / per * kPaM + at % per * a.G + g;
+    if (first < 0 || last >= blocks || at < 0 || at >= 2 * per) return;
+    for (int c0 = first; c0 <= last; c0 += 8) {
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t slot = 2 * (c0 + i) + (c0 + i == first);
+        ml[i] = c0 + i <= last ? __ldcg(a.ml + slot * 256 + row) : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t slot = 2 * (c0 + i) + (c0 + i == first);
+        if (ml[i].x != -INFINITY) x[i] = __ldcg(a.o + (slot * 32 + quad) * 256 + row);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) add(ml[i], x[i]);
     }
   };
+  auto begin = [&]() { m = -INFINITY, l = 0.f, o = make_float4(0.f, 0.f, 0.f, 0.f); };
+  auto finish = [&](int64_t tok, int qh) {
+    float den = l;
+    if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
+    const float inv = m == -INFINITY ? 0.f : 1.0f / den;
+    const uint2 w = make_uint2(pa_pack(o.x * inv, o.y * inv), pa_pack(o.z * inv, o.w * inv));
+    reinterpret_cast<uint2*>(a.out + tok * a.out_stride + qh * kPaD)[quad] = w;
+  };
   if (!a.group_starts) {
-    __syncthreads();
-    if (threadIdx.x == 0) a.rec[(int64_t)tok * a.Hkv + h].first = 0;
+    const PaSplit e = a.split[blockIdx.x / kPaJoin];
+    for (int r = (int)(blockIdx.x % kPaJoin) * 8 + sub; r < e.ntok * a.G; r += 8 * kPaJoin) {
+      const int at = r / a.G, g = r - at * a.G;
+      begin();
+      parts(e.first, e.last, at, g);
+      finish(e.tok0 + at, e.h * a.G + g);
+    }
+    return;
   }
-  if (own.prefix) parts(a.rec[((int64_t)a.batch + tok) * a.Hkv + h], 1);
-  parts(own, 0);
-  float den = l;
-  if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
-  const float inv = m == -INFINITY ? 0.f : 1.0f / den;
-  uint2 w = make_uint2(pa_pack(o.x * inv, o.y * inv), pa_pack(o.z * inv, o.w * inv));
-  reinterpret_cast<uint2*>(a.out + (int64_t)tok * a.out_stride + qh * kPaD)[quad] = w;
+  const int64_t r = (int64_t)blockIdx.x * 8 + sub;
+  const int Hq = a.Hkv * a.G;
+  if (r >= (int64_t)a.batch * Hq) return;
+  const int tok = (int)(r / Hq), qh = (int)(r - (int64_t)tok * Hq), h = qh / a.G;
+  const PaRecord own = a.rec[(int64_t)tok * a.Hkv + h];
+  if (own.first == PA_FINAL) return;
+  auto from = [&](const PaRecord& rec, int home) {
+    if (rec.first == PA_HOME) {
+      const int64_t row = (int64_t)(home * a.batch + tok) * Hq + qh;
+      const float2 ml = a.home_ml[row];
+      if (ml.x != -INFINITY) add(ml, a.home_o[row * 32 + quad]);
+    } else {
+      parts(rec.first, rec.last, tok - rec.tok0, qh - h * a.G);
+    }
+  };
+  begin();
+  if (own.prefix) from(a.rec[((int64_t)a.batch + tok) * a.Hkv + h], 1);
+  from(own, 0);
+  finish(tok, qh);
 }
 
 }  // namespace flint
@@ -1079,15 +1117,15 @@ using namespace flint;
 
 int64_t flint::status_offset_paged_attention() { return (int64_t)offsetof(PagedAttnWorkspace, status); }
 
-// The workspace: status, then (m, l) and o of the slots (two per block), of a size that the device alone decides; behind
-// them a prompt's records, which the join clears, so that they are clear for calls of any shape; or, with shared prefixes,
-// the homes and the records, which every call writes before it reads them.
+// The workspace: status, the blocks' cut items, (m, l) and o of their slots (two per block); with shared prefixes also the
+// homes and the records.  Every call writes what it reads.
 struct PaLayout {
-  int64_t ml, o, rec, home_ml, home_o, bytes;
+  int64_t split, ml, o, rec, home_ml, home_o, bytes;
 };
 static PaLayout pa_layout(int64_t blocks, int64_t records, int64_t homes) {
   PaLayout w;
-  w.ml = sizeof(PagedAttnWorkspace);
+  w.split = sizeof(PagedAttnWorkspace);
+  w.ml = w.split + (blocks * (int64_t)sizeof(PaSplit) + 127) / 128 * 128;
   w.o = w.ml + blocks * 512 * (int64_t)sizeof(float2);
   w.rec = w.o + blocks * 512 * 32 * (int64_t)sizeof(float4);
   w.home_o = w.rec + (records * (int64_t)sizeof(PaRecord) + 127) / 128 * 128;
@@ -1108,7 +1146,7 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   if (!q || !kv || !bt || !seq_lens || !out || !ws) return FLINT_ERR_ARGUMENT;
   if (window < 0 || window > INT32_MAX || !(scale > 0.f) || !(scale < 1e30f)) return FLINT_ERR_ARGUMENT;
   if (batch < 1 || batch > (1 << 20) || tokens < 1 || tokens > (1 << 24) || Hkv < 1 || Hkv > 128 || Hq < 1 || Hq % Hkv != 0 ||
-      Hq / Hkv > 8 || num_blocks < 1 || num_blocks >= INT32_MAX || max_blocks < 1 || max_blocks > (1 << 26) || bt_stride < 0 ||
+      Hq / Hkv > 8 || num_blocks < 1 || num_blocks >= INT32_MAX || max_blocks < 1 || max_blocks > (1 << 25) || bt_stride < 0 ||
       q_stride < Hq * kPaD || out_stride < Hq * kPaD || stride_head < kPaPage * 2 * kPaD || stride_block < kPaPage * 2 * kPaD)
     return FLINT_ERR_SHAPE;
   if (!aligned(kv, 16) || stride_block % 8 != 0 || stride_head % 8 != 0 || !aligned(out, 16) || !aligned(q, 16) ||
@@ -1133,8 +1171,9 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   a.window = (int)window; a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
   a.num_blocks = (int)num_blocks; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
   a.ws = static_cast<PagedAttnWorkspace*>(ws);
-  const PaLayout w = pa_layout(blocks, (group_starts ? 2 : 1) * tokens * Hkv, group_starts ? 2 * batch * Hq : 0);
+  const PaLayout w = pa_layout(blocks, group_starts ? 2 * batch * Hkv : 0, group_starts ? 2 * batch * Hq : 0);
   uint8_t* base = static_cast<uint8_t*>(ws);
+  a.split = reinterpret_cast<PaSplit*>(base + w.split);
   a.rec = reinterpret_cast<PaRecord*>(base + w.rec);
   a.ml = reinterpret_cast<float2*>(base + w.ml);
   a.o = reinterpret_cast<float4*>(base + w.o);
@@ -1151,13 +1190,14 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   }
   rc = launch(paged_attn_kernel, dim3((unsigned)blocks), dim3(kPaThreads), kPaSmem, stream, pdl, mq, mkv, a);
   if (rc) return rc;
-  return launch(paged_join_kernel, dim3((unsigned)tokens, (unsigned)Hkv), dim3(32 * G), 0, stream, pdl, a, blocks);
+  const int64_t grid = group_starts ? (batch * Hq + 7) / 8 : (int64_t)blocks * kPaJoin;
+  return launch(paged_join_kernel, dim3((unsigned)grid), dim3(256), 0, stream, pdl, a, blocks);
 }
 
 extern "C" int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads,
                                                            int64_t num_kv_heads) {
   if (batch < 1 || tokens < 1 || num_q_heads < 1 || num_kv_heads < 1) return -1;
-  return pa_layout(pa_blocks(), tokens * num_kv_heads, 0).bytes;
+  return pa_layout(pa_blocks(), 0, 0).bytes;
 }
 
 extern "C" int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_cache, int64_t num_blocks,
