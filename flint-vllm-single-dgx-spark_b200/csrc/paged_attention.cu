@@ -83,6 +83,7 @@ struct PagedAttnArgs {
   int groups;
   const float* sinks;
   int window, batch, tokens, Hkv, G, num_blocks;
+  int per, inv_g;                              // tokens of a row tile; 2^16 / G rounded up
   float c;
   bf16* out;
   int64_t out_stride;
@@ -276,6 +277,9 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile
   return pa_wait_long(bar, parity, failed, status);
 }
 
+// row / G of a row below 256 (exact: the error of inv_g is below 1 / 256 of a quotient's step)
+__device__ __forceinline__ int pa_token(const PagedAttnArgs& a, int row) { return (row * a.inv_g) >> 16; }
+
 // ---- the items ----
 // sum over i < k of max(0, a + i * t)
 __device__ __forceinline__ long long pa_ramp(int a, int t, int k) {
@@ -304,7 +308,7 @@ struct PaLine {
   const bool shared;
   const int per, tile;                         // tokens of a row tile, of an item
 
-  __device__ PaLine(const PagedAttnArgs& args) : a(args), shared(args.group_starts != nullptr), per(kPaM / args.G), tile(2 * per) {}
+  __device__ PaLine(const PagedAttnArgs& args) : a(args), shared(args.group_starts != nullptr), per(args.per), tile(2 * args.per) {}
   __device__ int segments() const { return shared ? a.groups + a.batch : a.batch; }
   __device__ void complain(bool bad) const {
     if (bad && blockIdx.x == 0) atomicOr(&a.ws->status, STATUS_BAD_SEQ);
@@ -448,8 +452,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   const int nseg = line.segments();
   long long* runs = reinterpret_cast<long long*>(ring);
   const int kept = (nseg + 31) / 32 <= kPaRuns ? (nseg + 31) / 32 : 0;
-  for (int i0 = 32 * warp; i0 < 32 * kept; i0 += kPaThreads) {
-    long long c = line.segment(i0 + lane).cost * a.Hkv;
+  PaSegment seg0;                                                 // the items' warp keeps its segment of the first run
+  for (int i0 = 32 * ((warp + 2) % 12); i0 < 32 * kept; i0 += kPaThreads) {
+    const PaSegment seg = line.segment(i0 + lane);
+    if (i0 == 0) seg0 = seg;
+    long long c = seg.cost * a.Hkv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
     if (lane == 0) runs[i0 / 32] = c;
@@ -486,7 +493,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           continue;
         }
       }
-      const PaSegment mine = line.segment(i0 + lane);
+      const PaSegment mine = kept && i0 == 0 ? seg0 : line.segment(i0 + lane);
       long long cum = mine.cost * a.Hkv;                          // inclusive scan over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -498,7 +505,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         at += chunk;
         continue;
       }
-      for (int k = 0; k < 32 && ok; ++k) {
+      // from the first segment that ends behind the share's start
+      const unsigned live = __ballot_sync(0xffffffffu, mine.cost > 0 && at + cum > x0);
+      for (int k = live ? __ffs(live) - 1 : 32; k < 32 && ok; ++k) {
         PaSegment s;
         s.tok0 = __shfl_sync(0xffffffffu, mine.tok0, k);
         s.ntok = __shfl_sync(0xffffffffu, mine.ntok, k);
@@ -629,7 +638,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       if (steps == 0) continue;
       const int* row = a.block_tables + (int64_t)it.table * a.bt_stride;
       const int pages_end = (it.end + kPaPage - 1) / kPaPage;
-      int held = -1, ids = 0;                                     // table entries of four steps, one per lane
+      // table entries of four steps, one per lane; the first ones are on their way while Q is sent for
+      int held = it.j0 >> 2, ids = it.begin / kPaPage + held * 32 + lane;
+      ids = ids < pages_end ? row[ids] : a.num_blocks;
       auto load = [&](int j, int column) {                        // step j's K (column 0) or V (column 128)
         const int p0 = it.begin / kPaPage + j * 8;
         if (held != j >> 2) {
@@ -659,7 +670,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       if (ok && !pa_wait(&b_q_free, (unsigned)((nq & 1) ^ 1), &s_failed, status)) ok = false;
       ++nq;
       if (ok && lane == 0) {
-        const int tiles = it.dual ? 2 : 1, per = kPaM / a.G;
+        const int tiles = it.dual ? 2 : 1, per = a.per;
         mbar_arrive_expect_tx(&b_q, (unsigned)(tiles * 2 * per * a.G * 128));
         for (int t = 0; t < tiles; ++t)
           for (int half = 0; half < 2; ++half)
@@ -788,10 +799,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
       if (it.ntok == 0) break;
-      const int per = kPaM / a.G, steps = it.j1 - it.j0;
-      const int tok = row / a.G + (it.dual ? t * per : 0);
-      const int qh = it.h * a.G + row % a.G;
-      const bool valid = row / a.G < per && tok < it.ntok;
+      const int per = a.per, steps = it.j1 - it.j0, row_tok = pa_token(a, row);
+      const int tok = row_tok + (it.dual ? t * per : 0);
+      const int qh = it.h * a.G + row - row_tok * a.G;
+      const bool valid = row_tok < per && tok < it.ntok;
       int lo = 0, hi = 0;                                         // this row's keys
       if (valid) {
         if (!it.home) hi = it.pos0 + tok + 1;
@@ -965,9 +976,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         if (it.out == PA_FINAL && (it.dual || t == 0)) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = 32 * (warp & 3) + 8 * i + (lane >> 2), tk = r / a.G + (it.dual ? t * per : 0);
-            to[i] = r / a.G < per && tk < it.ntok
-                        ? (int64_t)(it.tok0 + tk) * a.out_stride + (it.h * a.G + r % a.G) * kPaD + (lane & 3) * 8
+            const int r = 32 * (warp & 3) + 8 * i + (lane >> 2), rt = pa_token(a, r), tk = rt + (it.dual ? t * per : 0);
+            to[i] = rt < per && tk < it.ntok
+                        ? (int64_t)(it.tok0 + tk) * a.out_stride + (it.h * a.G + r - rt * a.G) * kPaD + (lane & 3) * 8
                         : -1;
           }
         }
@@ -1042,7 +1053,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
 constexpr int kPaJoin = 4;
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, int blocks) {
   pdl_wait();
-  const int sub = threadIdx.x & 7, quad = threadIdx.x >> 3, per = kPaM / a.G;
+  const int sub = threadIdx.x & 7, quad = threadIdx.x >> 3, per = a.per;
   float m, l;
   float4 o;
   auto add = [&](float2 ml, float4 x) {
@@ -1083,7 +1094,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, 
   if (!a.group_starts) {
     const PaSplit e = a.split[blockIdx.x / kPaJoin];
     for (int r = (int)(blockIdx.x % kPaJoin) * 8 + sub; r < e.ntok * a.G; r += 8 * kPaJoin) {
-      const int at = r / a.G, g = r - at * a.G;
+      const int at = pa_token(a, r), g = r - at * a.G;
       begin();
       parts(e.first, e.last, at, g);
       finish(e.tok0 + at, e.h * a.G + g);
@@ -1169,7 +1180,7 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   a.block_tables = bt; a.bt_stride = bt_stride; a.max_blocks = (int)max_blocks; a.cu_seqlens = cu_seqlens;
   a.seq_lens = seq_lens; a.group_starts = group_starts; a.prefix_lens = prefix_lens; a.groups = (int)groups; a.sinks = sinks;
   a.window = (int)window; a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
-  a.num_blocks = (int)num_blocks; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
+  a.num_blocks = (int)num_blocks; a.per = per; a.inv_g = (65536 + G - 1) / G; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
   a.ws = static_cast<PagedAttnWorkspace*>(ws);
   const PaLayout w = pa_layout(blocks, group_starts ? 2 * batch * Hkv : 0, group_starts ? 2 * batch * Hq : 0);
   uint8_t* base = static_cast<uint8_t*>(ws);
