@@ -9,8 +9,8 @@
 // 2^(sink log2 e - c m) to l.  A row without keys gives zeros.
 //
 // Work.  An item is one KV head and up to two row tiles of 128 rows: floor(128 / G) consecutive query tokens (or streams)
-// with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys,
-// doubled for two tiles, and a constant), the line is cut into equal shares, one per SM: a long prompt's items and a few
+// with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys and
+// a constant, for one tile as for two), the line is cut into equal shares, one per SM: a long prompt's items and a few
 // rows on a long cache are both split evenly, and where a cut falls into an item its parts leave (m, l, o) in the
 // workspace and a second launch joins them in the order of the keys.
 //   an item of two tiles: both tiles multiply the same keys; one's softmax runs under the other's products
@@ -51,11 +51,10 @@ constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA,
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaKey2 = 4, kPaKey1 = 3;        // cost of a key of an item of two / one tiles: 128 keys take 2.0 / 1.5 us,
-constexpr int kPaFixed2 = 1100, kPaFixed1 = 700;  // and of an item beside its keys: 4.3 / 2.7 us
-constexpr int kPaLeast = 800;                  // least share of a block
+constexpr int kPaFixed = 225;                  // cost of an item beside its keys, in keys (128 keys take some 1.9 us)
+constexpr int kPaLeast = 200;                  // least share of a block, in keys
 constexpr unsigned STATUS_BAD_SEQ = 4u;
-constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4 + 8 * 2048;
+constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4;
 
 struct PagedAttnWorkspace {
   unsigned status;
@@ -87,6 +86,7 @@ struct PagedAttnArgs {
   float c;
   bf16* out;
   int64_t out_stride;
+  int wide;                                    // rows of out begin at 32 bytes
   PagedAttnWorkspace* ws;
   PaSplit* split;                              // prompts: one for each block (ntok 0: none)
   PaRecord* rec;                               // shared prefixes: [batch][Hkv] own keys, then [batch][Hkv] prefixes
@@ -241,6 +241,20 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// 64 bytes of a row by one thread.  A row is a thread's: 32-byte stores fill a sector each; handing the columns round through
+// shared memory, so that a store covers whole lines, took twice as long (2.2 us an item, a chain of short steps).
+__device__ __forceinline__ void pa_store64(bf16* dst, const uint32_t* w, bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + 16 * i), "r"(w[8 * i]), "r"(w[8 * i + 1]),
+                   "r"(w[8 * i + 2]), "r"(w[8 * i + 3]), "r"(w[8 * i + 4]), "r"(w[8 * i + 5]), "r"(w[8 * i + 6]), "r"(w[8 * i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  }
+}
 __device__ __forceinline__ float pa_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -369,9 +383,6 @@ struct PaLine {
     const int p = s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
     return max(0, max(0, e) - max(s.lo, b));
   }
-  __device__ bool dual(const PaSegment& s, int i) const { return tokens_of(s, i) > per; }
-  __device__ int fixed(const PaSegment& s, int i) const { return dual(s, i) ? kPaFixed2 : kPaFixed1; }
-  __device__ long long weight(const PaSegment& s, int i) const { return (dual(s, i) ? (long long)kPaKey2 : kPaKey1) * keys(s, i); }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
     const int m = (s.ntok + tile - 1) / tile;
@@ -383,12 +394,11 @@ struct PaLine {
       w = pa_ramp(s.pos0 + tile, tile, whole);
       if (a.window > 0) w -= pa_ramp(s.pos0 - a.window + 1, tile, whole);
     }
-    w *= kPaKey2;
-    if (k >= m) w += weight(s, m - 1) + fixed(s, m - 1);
-    return w + (long long)kPaFixed2 * whole;
+    if (k >= m) w += keys(s, m - 1);
+    return w + (long long)kPaFixed * min(k, m);
   }
 };
-static_assert(kPaFixed1 > 0 && kPaFixed2 > 0, "every item has a place on the line");
+static_assert(kPaFixed > 0, "every item has a place on the line");
 
 __global__ void __launch_bounds__(kPaThreads, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const PagedAttnArgs a) {
@@ -396,7 +406,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;                                             // two Q tiles, each two halves of 64 columns
   uint8_t* ring = sq + 2 * kPaSlotBytes;
-  float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 32 columns of o between the halves; stores
+  float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 32 columns of o between the halves
   __shared__ PaItem items[kPaQueue];
   __shared__ __align__(8) uint64_t b_item[kPaQueue], b_item_free[kPaQueue], b_full[kPaSlots], b_empty[kPaSlots], b_q, b_q_free,
       b_s[2], b_p[4], b_o[2], b_hand, b_take;
@@ -533,12 +543,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             hi = min(hi, i + step);
           }
         }
-        long long start = seg0 + h * s.cost + line.upto(s, i), w = 0;
-        int fixed = 0;
+        long long start = seg0 + h * s.cost + line.upto(s, i);
+        int w = 0;
         for (; h < a.Hkv && ok && start < x1; ++h, i = 0)
-          for (; i < m && start < x1; ++i, start += fixed + w) {
-            w = line.weight(s, i), fixed = line.fixed(s, i);
-            const long long stop = start + fixed + w;
+          for (; i < m && start < x1; ++i, start += kPaFixed + w) {
+            w = line.keys(s, i);
+            const long long stop = start + kPaFixed + w;
             PaItem it;
             it.tok0 = s.tok0 + i * line.tile, it.ntok = line.tokens_of(s, i), it.h = h, it.table = s.table;
             it.dual = it.ntok > line.per;
@@ -566,7 +576,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             const unsigned unit = steps ? max(1u, ((unsigned)w + steps - 1) / (unsigned)steps) : 1u;
             auto before = [&](long long x) -> int {
               if (x >= stop) return steps;
-              return x <= start + fixed ? 0 : min(steps, (int)((unsigned)(x - start - fixed) / unit));
+              return x <= start + kPaFixed ? 0 : min(steps, (int)((unsigned)(x - start - kPaFixed) / unit));
             };
             it.j0 = before(x0), it.j1 = before(x1);
             PaRecord rec = {PA_NONE, PA_NONE, it.tok0, !s.home && s.lo > 0};
@@ -969,19 +979,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         const bool writes = valid && (it.dual || t == 0);
         const int64_t slot_row = it.out >= 0 ? (int64_t)it.out * 256 + (it.dual ? t * 128 : 0) + row : 0;
         const int64_t home_row = (int64_t)(it.home * a.batch + it.tok0 + tok) * a.Hkv * a.G + qh;
-        // Finished rows go out through shared memory, 32 columns of the warp's 32 rows at a time: lane k then writes 16 bytes
-        // of row 8 i + k / 4, so that a store covers 8 runs of 64 bytes and not 32 of 16.
-        uint4* stage = reinterpret_cast<uint4*>(sx + kPaM * 8) + warp * 128;
-        int64_t to[4];                                            // (-1: no such row)
-        if (it.out == PA_FINAL && (it.dual || t == 0)) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 32 * (warp & 3) + 8 * i + (lane >> 2), rt = pa_token(a, r), tk = rt + (it.dual ? t * per : 0);
-            to[i] = rt < per && tk < it.ntok
-                        ? (int64_t)(it.tok0 + tk) * a.out_stride + (it.h * a.G + r - rt * a.G) * kPaD + (lane & 3) * 8
-                        : -1;
-          }
-        }
+        bf16* dst = a.out + (int64_t)(it.tok0 + tok) * a.out_stride + qh * kPaD;
         float inv = 1.f;
 #pragma unroll 1
         for (int quarter = 0; quarter < 4; ++quarter) {
@@ -1008,23 +1006,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             }
           }
           if (it.out == PA_FINAL) {
+            if (writes) {
+              uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = m == -INFINITY ? 0u
-                                      : pa_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-              stage[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int i = 0; i < 16; ++i)
+                w[i] = m == -INFINITY ? 0u : pa_pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+              pa_store64(dst + 32 * quarter, w, a.wide);
             }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = 8 * i + (lane >> 2);
-              const uint4 w = stage[r * 4 + ((lane & 3) ^ ((r >> 1) & 3))];
-              if (to[i] >= 0) *reinterpret_cast<uint4*>(a.out + to[i] + 32 * quarter) = w;
-            }
-            __syncwarp();
           } else if (writes && m != -INFINITY) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -1181,6 +1169,7 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   a.seq_lens = seq_lens; a.group_starts = group_starts; a.prefix_lens = prefix_lens; a.groups = (int)groups; a.sinks = sinks;
   a.window = (int)window; a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
   a.num_blocks = (int)num_blocks; a.per = per; a.inv_g = (65536 + G - 1) / G; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
+  a.wide = aligned(out, 32) && out_stride % 16 == 0;
   a.ws = static_cast<PagedAttnWorkspace*>(ws);
   const PaLayout w = pa_layout(blocks, group_starts ? 2 * batch * Hkv : 0, group_starts ? 2 * batch * Hq : 0);
   uint8_t* base = static_cast<uint8_t*>(ws);
