@@ -188,15 +188,14 @@ def workspace(device: torch.device, kind: str, nbytes: int) -> torch.Tensor:
 _last_raw: dict[tuple[int, str], int] = {}      # the same, as raw handles: what workspace_and_stream looks at first
 
 
-def workspace_and_stream(device: torch.device, kind: str, nbytes: int) -> tuple[int, int]:
-    """-> (address of workspace(device, kind, nbytes), the current stream's handle).  Where the stream is the one that
-    used the workspace last and the workspace is large enough there is nothing to order or allocate, and none of the
+def workspace_and_stream(index: int, kind: str, nbytes: int) -> tuple[int, int]:
+    """-> (address of the workspace `kind` of device `index`, the current stream's handle).  Where the stream is the one
+    that used the workspace last and the workspace is large enough there is nothing to order or allocate, and none of the
     stream objects that workspace() needs is made (8 us of host time a call)."""
-    index = device.index if device.index is not None else torch.cuda.current_device()
     key, raw = (index, kind), torch._C._cuda_getCurrentRawStream(index)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes or _last_raw.get(key) != raw:
-        ws = workspace(device, kind, nbytes)
+        ws = workspace(torch.device("cuda", index), kind, nbytes)
         if not torch.cuda.is_current_stream_capturing():
             _last_raw[key] = raw
     return ws.data_ptr(), raw

@@ -45,7 +45,7 @@ constexpr int kPaSlots = 4;                    // ring slots of 128 keys x 128 c
 constexpr int kPaSlotBytes = kPaKeys * kPaD * 2;
 constexpr int kPaHalf = kPaSlotBytes / 2;      // 64 columns
 constexpr int kPaPageHalf = kPaPage * 128;     // a page's 64 columns
-constexpr int kPaRuns = 2048;                  // runs of 32 segments whose costs are kept
+constexpr int kPaRuns = 64;                    // runs of 32 segments that are kept
 constexpr int kPaQueue = 4;                    // items cut ahead
 constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA, items, one idle
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
@@ -377,11 +377,14 @@ struct PaLine {
     return s;
   }
   __device__ int tokens_of(const PaSegment& s, int i) const { return min(tile, s.ntok - i * tile); }
-  // keys that item i is taken to cost
+  // keys that item i is taken to cost; a segment of one item, as a stream's own keys are, in whole steps
   __device__ int keys(const PaSegment& s, int i) const {
-    if (s.home) return a.window > 0 ? min(s.hi, a.window) : s.hi;
-    const int p = s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
-    return max(0, max(0, e) - max(s.lo, b));
+    int n = a.window > 0 ? min(s.hi, a.window) : s.hi;
+    if (!s.home) {
+      const int p = s.pos0 + i * tile, e = p + tokens_of(s, i), b = a.window > 0 ? p - a.window + 1 : 0;
+      n = max(0, max(0, e) - max(s.lo, b));
+    }
+    return s.ntok <= tile ? (n + kPaKeys - 1) & ~(kPaKeys - 1) : n;
   }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
@@ -461,26 +464,24 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   const PaLine line(a);
   const int nseg = line.segments();
   long long* runs = reinterpret_cast<long long*>(ring);
-  const int kept = (nseg + 31) / 32 <= kPaRuns ? (nseg + 31) / 32 : 0;
-  PaSegment seg0;                                                 // the items' warp keeps its segment of the first run
+  PaSegment* segs = reinterpret_cast<PaSegment*>(runs + kPaRuns);
+  const int kept = nseg <= 32 * kPaRuns ? (nseg + 31) / 32 : 0;
   for (int i0 = 32 * ((warp + 2) % 12); i0 < 32 * kept; i0 += kPaThreads) {
     const PaSegment seg = line.segment(i0 + lane);
-    if (i0 == 0) seg0 = seg;
+    segs[i0 + lane] = seg;
     long long c = seg.cost * a.Hkv;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
     if (lane == 0) runs[i0 / 32] = c;
   }
   __syncthreads();
-  long long total = 0, my_run = 0;
-  if (warp == 10) {                                               // (read before the ring fills)
-    for (int i = lane; i < kept; i += 32) total += runs[i];
-    my_run = lane < kept ? runs[lane] : 0;
-  }
-  __syncthreads();
 
   if (warp == 10) {
     // ---- items: this block's share of the line ----
+    // (what the others left in the ring is read until the first item goes out: the TMA warp fills it after that)
+    long long total = 0, my_run[2];
+    for (int i = lane; i < kept; i += 32) total += runs[i];
+    for (int i = 0; i < 2; ++i) my_run[i] = lane + 32 * i < kept ? runs[lane + 32 * i] : 0;
     if (!kept)
       for (int i0 = 0; i0 < nseg; i0 += 32) total += line.segment(i0 + lane).cost * a.Hkv;
 #pragma unroll
@@ -496,14 +497,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     bool ok = true;
     PaSplit cut_item = {};
     for (int i0 = 0; i0 < nseg && at < x1 && ok; i0 += 32) {
-      if (kept && i0 < 32 * 32) {                                 // a run before the share
-        const long long c = __shfl_sync(0xffffffffu, my_run, i0 / 32);
+      if (kept) {                                                 // a run before the share
+        const long long c = __shfl_sync(0xffffffffu, my_run[i0 / 1024], i0 / 32 % 32);
         if (at + c <= x0) {
           at += c;
           continue;
         }
       }
-      const PaSegment mine = kept && i0 == 0 ? seg0 : line.segment(i0 + lane);
+      const PaSegment mine = kept && n_items == 0 ? segs[i0 + lane] : line.segment(i0 + lane);
       long long cum = mine.cost * a.Hkv;                          // inclusive scan over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -1035,13 +1036,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kPaTmem) : "memory");
 }
 
-// Joins the parts of the rows that were cut: 8 rows at a time, a thread per row and quad of columns.  Prompts: kPaJoin
-// blocks for each item that was cut; streams: a block for 8 of their rows.  Parts are added in the order of their keys, the
-// prefix first; their (m, l), then their o, are loaded eight at a time, since what this costs is the latency of L2.
-constexpr int kPaJoin = 4;
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, int blocks) {
+// Joins the parts of the rows that were cut, the prefix's first, in the order of their keys: 8 / Groups rows at a time, a
+// thread per row, quad of columns and group of parts (every Groups-th); the groups' sums are joined in their order.  Prompts:
+// kPaJoin blocks for each item that was cut; streams: a block for 8 / Groups of their rows.  Parts' (m, l), then their o, are
+// loaded four at a time, since what this costs is the latency of L2.
+constexpr int kPaJoin = 8;
+template <int Groups>
+__global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedAttnArgs a, int blocks) {
+  constexpr int kRows = 8 / Groups;
+  __shared__ float4 s_o[Groups > 1 ? 256 : 1];
+  __shared__ float2 s_ml[Groups > 1 ? 8 : 1];
   pdl_wait();
-  const int sub = threadIdx.x & 7, quad = threadIdx.x >> 3, per = a.per;
+  const int sub = threadIdx.x & 7, quad = threadIdx.x >> 3, row_in = sub % kRows, group = sub / kRows, per = a.per;
   float m, l;
   float4 o;
   auto add = [&](float2 ml, float4 x) {
@@ -1054,25 +1060,35 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, 
   auto parts = [&](int first, int last, int at, int g) {          // at: the token's place in its item
     const int row = at / per * kPaM + at % per * a.G + g;
     if (first < 0 || last >= blocks || at < 0 || at >= 2 * per) return;
-    for (int c0 = first; c0 <= last; c0 += 8) {
-      float2 ml[8];
-      float4 x[8];
+    for (int c0 = first + group; c0 <= last; c0 += 4 * Groups) {
+      float2 ml[4];
+      float4 x[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t slot = 2 * (c0 + i) + (c0 + i == first);
-        ml[i] = c0 + i <= last ? __ldcg(a.ml + slot * 256 + row) : make_float2(-INFINITY, 0.f);
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * Groups;
+        ml[i] = c <= last ? __ldcg(a.ml + (2 * c + (c == first)) * 256 + row) : make_float2(-INFINITY, 0.f);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t slot = 2 * (c0 + i) + (c0 + i == first);
-        if (ml[i].x != -INFINITY) x[i] = __ldcg(a.o + (slot * 32 + quad) * 256 + row);
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + i * Groups;
+        if (ml[i].x != -INFINITY) x[i] = __ldcg(a.o + ((2 * c + (c == first)) * 32 + quad) * 256 + row);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) add(ml[i], x[i]);
+      for (int i = 0; i < 4; ++i) add(ml[i], x[i]);
     }
   };
   auto begin = [&]() { m = -INFINITY, l = 0.f, o = make_float4(0.f, 0.f, 0.f, 0.f); };
-  auto finish = [&](int64_t tok, int qh) {
+  auto finish = [&](bool valid, int64_t tok, int qh) {            // every thread of the block
+    if (Groups > 1) {
+      if (quad == 0) s_ml[sub] = make_float2(m, l);
+      s_o[quad * 8 + sub] = o;
+      __syncthreads();
+      if (group == 0)
+#pragma unroll
+        for (int k = 1; k < Groups; ++k) add(s_ml[k * kRows + row_in], s_o[quad * 8 + k * kRows + row_in]);
+      __syncthreads();
+    }
+    if (!valid || group != 0) return;
     float den = l;
     if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
     const float inv = m == -INFINITY ? 0.f : 1.0f / den;
@@ -1081,33 +1097,36 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnArgs a, 
   };
   if (!a.group_starts) {
     const PaSplit e = a.split[blockIdx.x / kPaJoin];
-    for (int r = (int)(blockIdx.x % kPaJoin) * 8 + sub; r < e.ntok * a.G; r += 8 * kPaJoin) {
-      const int at = pa_token(a, r), g = r - at * a.G;
+    const int rows = e.ntok * a.G;
+    for (int r0 = (int)(blockIdx.x % kPaJoin) * kRows; r0 < rows; r0 += kRows * kPaJoin) {
+      const int r = r0 + row_in, at = pa_token(a, r), g = r - at * a.G;
       begin();
-      parts(e.first, e.last, at, g);
-      finish(e.tok0 + at, e.h * a.G + g);
+      if (r < rows) parts(e.first, e.last, at, g);
+      finish(r < rows, e.tok0 + at, e.h * a.G + g);
     }
     return;
   }
-  const int64_t r = (int64_t)blockIdx.x * 8 + sub;
+  const int64_t r = (int64_t)blockIdx.x * kRows + row_in;
   const int Hq = a.Hkv * a.G;
-  if (r >= (int64_t)a.batch * Hq) return;
-  const int tok = (int)(r / Hq), qh = (int)(r - (int64_t)tok * Hq), h = qh / a.G;
+  const bool valid = r < (int64_t)a.batch * Hq;
+  const int tok = valid ? (int)(r / Hq) : 0, qh = valid ? (int)(r - (int64_t)tok * Hq) : 0, h = qh / a.G;
   const PaRecord own = a.rec[(int64_t)tok * a.Hkv + h];
-  if (own.first == PA_FINAL) return;
+  const bool todo = valid && own.first != PA_FINAL;
   auto from = [&](const PaRecord& rec, int home) {
-    if (rec.first == PA_HOME) {
+    if (rec.first != PA_HOME) {
+      parts(rec.first, rec.last, tok - rec.tok0, qh - h * a.G);
+    } else if (group == 0) {
       const int64_t row = (int64_t)(home * a.batch + tok) * Hq + qh;
       const float2 ml = a.home_ml[row];
       if (ml.x != -INFINITY) add(ml, a.home_o[row * 32 + quad]);
-    } else {
-      parts(rec.first, rec.last, tok - rec.tok0, qh - h * a.G);
     }
   };
   begin();
-  if (own.prefix) from(a.rec[((int64_t)a.batch + tok) * a.Hkv + h], 1);
-  from(own, 0);
-  finish(tok, qh);
+  if (todo) {
+    if (own.prefix) from(a.rec[((int64_t)a.batch + tok) * a.Hkv + h], 1);
+    from(own, 0);
+  }
+  finish(todo, tok, qh);
 }
 
 }  // namespace flint
@@ -1190,8 +1209,13 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   }
   rc = launch(paged_attn_kernel, dim3((unsigned)blocks), dim3(kPaThreads), kPaSmem, stream, pdl, mq, mkv, a);
   if (rc) return rc;
-  const int64_t grid = group_starts ? (batch * Hq + 7) / 8 : (int64_t)blocks * kPaJoin;
-  return launch(paged_join_kernel, dim3((unsigned)grid), dim3(256), 0, stream, pdl, a, blocks);
+  // Few rows are cut into many parts, which four groups share (8 streams on a 6,048-token prefix, 256 rows in some 30 parts:
+  // 28 us a call against 31); many rows keep the SMs full by themselves (6,057 tokens: 294 us against 347).
+  const int64_t rows = (group_starts ? batch : tokens) * Hq;
+  const int per_block = rows <= (group_starts ? 4096 : 256) ? 2 : 8;
+  const dim3 grid((unsigned)(group_starts ? (rows + per_block - 1) / per_block : (int64_t)blocks * kPaJoin));
+  return per_block == 2 ? launch(paged_join_kernel<4>, grid, dim3(256), 0, stream, pdl, a, blocks)
+                        : launch(paged_join_kernel<1>, grid, dim3(256), 0, stream, pdl, a, blocks);
 }
 
 extern "C" int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads,

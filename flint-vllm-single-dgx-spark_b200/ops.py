@@ -9,6 +9,7 @@ their workspaces exist (see ``_lib.workspace``).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -846,7 +847,7 @@ def _check_paged(what, q, kv, bt, seq_lens, sinks, out):
     """Shapes and types that the prompt and shared-prefix attention have in common -> the C ABI's arguments up to the
     block tables, out's row stride.  (The stride of a dimension of one element says nothing and is not looked at.)"""
     _lib.require_cuda(q, what)
-    dev, shape, kv_shape, bt_shape = q.device, q.shape, kv.shape, bt.shape
+    shape, kv_shape, bt_shape, dev = q.shape, kv.shape, bt.shape, q.get_device()
     qs, os, ks = q.stride(), out.stride(), kv.stride()
     if len(shape) != 3 or shape[2] != 128 or q.dtype != _BF16 or qs[2] != 1 or (qs[1] != 128 and shape[1] != 1):
         raise _lib.FlintError(f"{what}: q must be bf16 [rows, heads, 128] with contiguous heads, got {q.dtype} "
@@ -854,7 +855,7 @@ def _check_paged(what, q, kv, bt, seq_lens, sinks, out):
     T, Hq, _ = shape
     if out.shape != shape or out.dtype != _BF16 or os[2] != 1 or (os[1] != 128 and Hq != 1):
         raise _lib.FlintError(f"{what}: out must be bf16 {tuple(shape)} with contiguous heads")
-    if len(kv_shape) != 4 or kv_shape[2:] != (16, 256) or kv.dtype != _BF16 or ks[3] != 1 or ks[2] != 256:
+    if len(kv_shape) != 4 or kv_shape[2] != 16 or kv_shape[3] != 256 or kv.dtype != _BF16 or ks[3] != 1 or ks[2] != 256:
         raise _lib.FlintError(f"{what}: kv_cache must be HND bf16 [blocks, kv_heads, 16, 256]")
     nblk, Hkv, _, _ = kv_shape
     if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= 8:
@@ -864,10 +865,10 @@ def _check_paged(what, q, kv, bt, seq_lens, sinks, out):
         raise _lib.FlintError(f"{what}: block_tables must be int32 [batch, max_blocks] with rows contiguous, seq_lens "
                               "int32 [batch]")
     if sinks is not None and (sinks.dtype != _F32 or sinks.numel() != Hq or not sinks.is_contiguous()
-                              or sinks.device != dev):
-        raise _lib.FlintError(f"{what}: sinks must be fp32 [{Hq}] on {dev}")
-    if kv.device != dev or bt.device != dev or seq_lens.device != dev or out.device != dev:
-        raise _lib.FlintError(f"{what}: all tensors must be on {dev}")
+                              or sinks.get_device() != dev):
+        raise _lib.FlintError(f"{what}: sinks must be fp32 [{Hq}] on {q.device}")
+    if kv.get_device() != dev or bt.get_device() != dev or seq_lens.get_device() != dev or out.get_device() != dev:
+        raise _lib.FlintError(f"{what}: all tensors must be on {q.device}")
     row = Hq * 128
     return ((q.data_ptr(), qs[0] if T > 1 else row, kv.data_ptr(), nblk, Hkv, ks[0] if nblk > 1 else Hkv * 4096,
              ks[1] if Hkv > 1 else 4096, bt.data_ptr(), bt.stride(0) if bt_shape[0] > 1 else bt_shape[1], bt_shape[1]),
@@ -875,8 +876,15 @@ def _check_paged(what, q, kv, bt, seq_lens, sinks, out):
 
 
 def _check_int32(what, name, t, n, dev):
-    if t.dtype != _I32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
-        raise _lib.FlintError(f"{what}: {name} must be int32 [{n}] on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype != _I32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
+        raise _lib.FlintError(f"{what}: {name} must be int32 [{n}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on "
+                              f"{t.device}")
+
+
+@functools.lru_cache(maxsize=256)
+def _bytes_of(fn: str, *sizes) -> int:
+    """A workspace's size: a function of the sizes alone."""
+    return int(getattr(lib(), fn)(*sizes))
 
 
 def _prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -885,13 +893,13 @@ def _prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: to
     """Causal attention of packed query tokens over the paged cache (flint_prefill_attention)."""
     args, out_stride = _check_paged("prefill_attention", q, kv_cache, block_tables, seq_lens, sinks, out)
     T, Hq, _ = q.shape
-    B, dev = seq_lens.shape[0], q.device
+    B, dev = seq_lens.shape[0], q.get_device()
     _check_int32("prefill_attention", "cu_seqlens", cu_seqlens, B + 1, dev)
     if T == 0 or B == 0:
         return
     L = lib()
     ws, stream = _lib.workspace_and_stream(dev, "prefill_attention",
-                                           L.flint_prefill_attention_workspace_bytes(B, T, Hq, args[4]))
+                                           _bytes_of("flint_prefill_attention_workspace_bytes", B, T, Hq, args[4]))
     rc = L.flint_prefill_attention(*args, cu_seqlens.data_ptr(), seq_lens.data_ptr(), ptr(sinks), window, scale, B, T, Hq,
                                    out.data_ptr(), out_stride, ws, PDL, stream)
     if rc:
@@ -913,7 +921,7 @@ def _shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     what = "shared_prefix_attention"
     args, out_stride = _check_paged(what, q, kv_cache, block_tables, seq_lens, sinks, out)
     B, Hq, _ = q.shape
-    n, dev = prefix_lens.numel(), q.device
+    n, dev = prefix_lens.numel(), q.get_device()
     if seq_lens.shape[0] != B:
         raise _lib.FlintError(f"{what}: {B} queries, {seq_lens.shape[0]} seq_lens")
     _check_int32(what, "prefix_lens", prefix_lens, n, dev)
@@ -921,7 +929,8 @@ def _shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     if B == 0:
         return
     L = lib()
-    ws, stream = _lib.workspace_and_stream(dev, what, L.flint_shared_prefix_attention_workspace_bytes(B, n, Hq, args[4]))
+    ws, stream = _lib.workspace_and_stream(dev, what, _bytes_of("flint_shared_prefix_attention_workspace_bytes", B, n, Hq,
+                                                                args[4]))
     rc = L.flint_shared_prefix_attention(*args, seq_lens.data_ptr(), group_starts.data_ptr(), prefix_lens.data_ptr(), n,
                                          ptr(sinks), window, scale, B, Hq, out.data_ptr(), out_stride, ws, PDL, stream)
     if rc:
@@ -943,12 +952,12 @@ def _(q, kv_cache, block_tables, seq_lens, group_starts, prefix_lens, sinks, win
 def _check_pool(what, ref, bt, seq_lens, num_pages):
     """-> the C ABI's arguments ref .. num_streams, and those of the workspace and stream."""
     _lib.require_cuda(ref, what)
-    dev, blocks, S, bt_shape = ref.device, ref.numel(), num_pages.numel(), bt.shape
+    dev, blocks, S, bt_shape = ref.get_device(), ref.numel(), num_pages.numel(), bt.shape
     _check_int32(what, "ref", ref, blocks, dev)
     _check_int32(what, "num_pages", num_pages, S, dev)
     if (bt.dtype != _I32 or len(bt_shape) != 2 or bt_shape[0] != S or (bt.stride(1) != 1 and bt_shape[1] != 1)
-            or bt.device != dev):
-        raise _lib.FlintError(f"{what}: block_tables must be int32 [{S}, max_blocks] with rows contiguous on {dev}")
+            or bt.get_device() != dev):
+        raise _lib.FlintError(f"{what}: block_tables must be int32 [{S}, max_blocks] with rows contiguous on {ref.device}")
     args = (ref.data_ptr(), blocks, bt.data_ptr(), bt.stride(0) if S > 1 else bt_shape[1], bt_shape[1])
     if seq_lens is not None:
         _check_int32(what, "seq_lens", seq_lens, S, dev)
@@ -959,15 +968,16 @@ def _check_pool(what, ref, bt, seq_lens, num_pages):
 def _check_kv(what, kv, ref):
     """-> the C ABI's arguments kv .. stride_block."""
     shape, st = kv.shape, kv.stride()
-    if (len(shape) != 5 or shape[3:] != (16, 256) or kv.dtype != _BF16 or kv.device != ref.device
+    if (len(shape) != 5 or shape[3] != 16 or shape[4] != 256 or kv.dtype != _BF16 or kv.get_device() != ref.get_device()
             or shape[1] != ref.numel() or st[4] != 1 or st[3] != 256 or (st[2] != 4096 and shape[2] != 1)):
         raise _lib.FlintError(f"{what}: kv must be bf16 [layers, {ref.numel()}, kv_heads, 16, 256] with contiguous pages")
     page = shape[2] * 4096
     return (kv.data_ptr(), shape[0], shape[2], st[0] if shape[0] > 1 else page * shape[1], st[1] if shape[1] > 1 else page)
 
 
-def _pages_ws(L, ref):
-    ws, stream = _lib.workspace_and_stream(ref.device, "kv_pages", L.flint_kv_pages_workspace_bytes(ref.numel()))
+def _pages_ws(ref):
+    ws, stream = _lib.workspace_and_stream(ref.get_device(), "kv_pages",
+                                           _bytes_of("flint_kv_pages_workspace_bytes", ref.numel()))
     return ws, PDL, stream
 
 
@@ -975,11 +985,11 @@ def _kv_reserve(ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.
                 lens: torch.Tensor) -> None:
     """Pages for streams up to lens tokens (flint_kv_reserve)."""
     pool, n, L = _check_pool("kv_reserve", ref, block_tables, None, num_pages), streams.numel(), lib()
-    _check_int32("kv_reserve", "streams", streams, n, ref.device)
-    _check_int32("kv_reserve", "lens", lens, n, ref.device)
+    _check_int32("kv_reserve", "streams", streams, n, ref.get_device())
+    _check_int32("kv_reserve", "lens", lens, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_reserve(*pool, streams.data_ptr(), lens.data_ptr(), n, *_pages_ws(L, ref))
+    rc = L.flint_kv_reserve(*pool, streams.data_ptr(), lens.data_ptr(), n, *_pages_ws(ref))
     if rc:
         check(rc, "flint_kv_reserve")
 
@@ -997,11 +1007,11 @@ def _kv_fork(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, se
     """Streams dst become copies of src, whole pages shared (flint_kv_fork)."""
     pool, n, L = _check_pool("kv_fork", ref, block_tables, seq_lens, num_pages), src.numel(), lib()
     cache = _check_kv("kv_fork", kv, ref)
-    _check_int32("kv_fork", "src", src, n, ref.device)
-    _check_int32("kv_fork", "dst", dst, n, ref.device)
+    _check_int32("kv_fork", "src", src, n, ref.get_device())
+    _check_int32("kv_fork", "dst", dst, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_fork(*cache, *pool, src.data_ptr(), dst.data_ptr(), n, *_pages_ws(L, ref))
+    rc = L.flint_kv_fork(*cache, *pool, src.data_ptr(), dst.data_ptr(), n, *_pages_ws(ref))
     if rc:
         check(rc, "flint_kv_fork")
 
@@ -1019,10 +1029,10 @@ def _kv_free(ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tens
              streams: torch.Tensor) -> None:
     """Streams give their pages back (flint_kv_free)."""
     pool, n, L = _check_pool("kv_free", ref, block_tables, seq_lens, num_pages), streams.numel(), lib()
-    _check_int32("kv_free", "streams", streams, n, ref.device)
+    _check_int32("kv_free", "streams", streams, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_free(*pool, streams.data_ptr(), n, *_pages_ws(L, ref))
+    rc = L.flint_kv_free(*pool, streams.data_ptr(), n, *_pages_ws(ref))
     if rc:
         check(rc, "flint_kv_free")
 
@@ -1041,9 +1051,9 @@ def _kv_compact(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor,
     """Used pages to the front of the pool (flint_kv_compact)."""
     pool, L = _check_pool("kv_compact", ref, block_tables, None, num_pages), lib()
     cache = _check_kv("kv_compact", kv, ref)
-    _check_int32("kv_compact", "remap", remap, ref.numel(), ref.device)
-    _check_int32("kv_compact", "live", live, 1, ref.device)
-    rc = L.flint_kv_compact(*cache, *pool, remap.data_ptr(), live.data_ptr(), *_pages_ws(L, ref))
+    _check_int32("kv_compact", "remap", remap, ref.numel(), ref.get_device())
+    _check_int32("kv_compact", "live", live, 1, ref.get_device())
+    rc = L.flint_kv_compact(*cache, *pool, remap.data_ptr(), live.data_ptr(), *_pages_ws(ref))
     if rc:
         check(rc, "flint_kv_compact")
 
