@@ -17,6 +17,12 @@ also the small case used for full ncu captures of one kernel.
 times the checkpoint-format kernels on one tensor of --rows x --cols values (default: the LM head, 174.6 MB of GGUF
 bytes, larger than L2).
 
+    python kernel_bench.py --kernel prefill_attention [--tokens 6057] [--ctx 0]
+    python kernel_bench.py --kernel shared_prefix_attention [--batch 8] [--ctx 6057]
+
+times the attention of one layer over a prompt of --tokens tokens behind --ctx cached ones (0: a whole prompt), or of
+--batch streams that share a prefix of --ctx tokens and are up to 200 tokens behind it.
+
     python flint-vllm-single-dgx-spark_b200/build.py --timeline _build_tl
     python kernel_bench.py --lib _build_tl/libflint_b200.so --timeline --kernel moe_fused --moe fused --batch 8
 
@@ -73,6 +79,10 @@ TIMELINES = {
         14: "producer: last stage", 9: "down tiles done", 10: "barrier 2", 11: "output written"}),
 }
 TIMELINES["moe_block_shared"] = TIMELINES["moe_block"]
+TIMELINES["prefill_attention"] = TIMELINES["shared_prefix_attention"] = ("flint_timeline_paged_attention", {
+    0: "entry", 1: "barriers, tensor memory", 2: "PDL wait done", 3: "cost of all items known", 4: "first item posted",
+    5: "first keys requested", 6: "Q landed", 7: "first scores", 8: "first probabilities", 9: "first item's sums complete",
+    10: "first item written", 11: "block done"})
 TIMELINES["moe_fused_ep"] = TIMELINES["moe_fused"]
 
 
@@ -106,7 +116,7 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", required=True, help="a layer op name (attn_block, moe_block, route, ...), head, "
                     "head_sample, or all")
-    ap.add_argument("--ctx", type=int, default=6057)
+    ap.add_argument("--ctx", type=int, default=None, help="default 6057 (prefill_attention: 0)")
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--reps", type=int, default=5)
     ap.add_argument("--batch", type=int, default=1)
@@ -123,11 +133,15 @@ def main(argv=None):
     ap.add_argument("--lib", default=None, help="load this build of libflint_b200.so (e.g. an instrumented one)")
     ap.add_argument("--timeline", action="store_true", help="print the kernel's phase stamps (instrumented build)")
     args = ap.parse_args(argv)
+    if args.ctx is None:
+        args.ctx = 0 if args.kernel == "prefill_attention" else 6057
     _package(args.lib)
     if args.kernel in ("gguf_repack", "nvfp4_dequant"):
         return time_format_kernel(args)
     if args.kernel == "grouped_moe":
         return time_grouped_moe(args)
+    if args.kernel in ("prefill_attention", "shared_prefix_attention"):
+        return time_paged_attention(args)
     from flint_b200.model import Decoder, FlintConfig, FlintModel
 
     cfg = FlintConfig(layers=args.layers) if args.config == "baseline" else FlintConfig.flint(layers=args.layers)
@@ -224,6 +238,59 @@ def time_grouped_moe(args):
     wbytes = E * (2 * I * H + H * I) * 9 // 16
     print(json.dumps({"kernel": "grouped_moe", "tokens": T, "experts": E, "topk": k, "ms_per_layer": res,
                       "expert_weight_bytes": wbytes}), flush=True)
+
+
+def time_paged_attention(args):
+    """flint_prefill_attention of one sequence, or flint_shared_prefix_attention of one group: 32 heads on 4 KV heads,
+    scattered pages, N(0, 1) values; a graph of --reps calls, CUDA events around its replay."""
+    from flint_b200.prefill_attention import flint_prefill_attention
+    from flint_b200.shared_prefix_attention import flint_shared_prefix_attention
+    dev = torch.device("cuda", torch.cuda.current_device())
+    g = torch.Generator(device=dev).manual_seed(13)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    prefill = args.kernel == "prefill_attention"
+    first = args.ctx // 16
+    lens = [args.ctx + args.tokens] if prefill else [args.ctx + 1 + 53 * b % 200 for b in range(args.batch)]
+    rows = args.tokens if prefill else args.batch
+    shared = 0 if prefill else first
+    own = [-(-n // 16) - shared for n in lens]
+    ids = torch.randperm(shared + sum(own), device=dev, generator=g).tolist()
+    prefix = [ids.pop() for _ in range(shared)]
+    width = max(own)
+    tables = i32([prefix + [ids.pop() for _ in range(n)] + [0] * (width - n) for n in own])
+    kv = torch.randn((shared + sum(own), 4, 16, 256), device=dev, generator=g, dtype=torch.bfloat16)
+    q = torch.randn((rows, 32, 128), device=dev, generator=g, dtype=torch.bfloat16)
+    out, n, scale = torch.empty_like(q), i32(lens), 128 ** -0.5
+    if prefill:
+        cu = i32([0, rows])
+        fn = lambda: flint_prefill_attention(q, kv, tables, cu, n, None, None, scale, out)
+        pairs = rows * args.ctx + rows * (rows + 1) // 2
+        nbytes = 2 * q.numel() * 2 + lens[0] * 4 * 512
+    else:
+        starts, plen = i32([0, rows]), i32([16 * first])
+        fn = lambda: flint_shared_prefix_attention(q, kv, tables, n, starts, plen, None, None, scale, out)
+        pairs = sum(lens)
+        nbytes = 2 * q.numel() * 2 + (16 * first + sum(x - 16 * first for x in lens)) * 4 * 512
+    fn()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(args.reps):
+            fn()
+    graph.replay()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    graph.replay()
+    e1.record()
+    torch.cuda.synchronize()
+    us = e0.elapsed_time(e1) * 1e3 / args.reps
+    flops = 4 * 128 * 32 * pairs
+    print(json.dumps({"kernel": args.kernel, "rows": rows, "ctx": args.ctx, "us_per_call": round(us, 2), "bytes": nbytes,
+                      "GBps": round(nbytes / us / 1e3, 1), "TFLOPs": round(flops / us / 1e6, 1)}), flush=True)
+    if args.timeline:
+        print_timeline(args.kernel)
+    del graph
 
 
 def time_format_kernel(args):
