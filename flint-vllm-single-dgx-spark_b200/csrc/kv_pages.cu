@@ -46,6 +46,10 @@ __device__ __forceinline__ int4* pg_fork_plan(const KvPool& p) { return reinterp
 __device__ __forceinline__ int* pg_fork_tail(const KvPool& p) { return reinterpret_cast<int*>(pg_fork_plan(p) + kPgMaxRequests); }
 __device__ __forceinline__ int2* pg_moves(const KvPool& p) { return reinterpret_cast<int2*>(p.ws + 1); }
 
+// Kernels that follow may look at tables, lengths and old pages before their wait on this grid (the decode attention does):
+// they are started when its last block ends, so each block ends with its writes in place.
+__device__ __forceinline__ void pg_publish() { __threadfence(); }
+
 // The sum of v over the planning block and, in *before, over the threads ahead of this one.
 __device__ __forceinline__ int pg_scan(int v, int* before, int* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -118,6 +122,7 @@ __global__ void __launch_bounds__(256) kv_free_kernel(const KvPool p, const int*
       atomicOr(&p.ws->status, STATUS_BAD_STREAM);
     }
   }
+  pg_publish();
 }
 
 // One block.  Stream streams[i] gets pages up to lens[i] tokens; a demand beyond the free pages is refused whole.
@@ -174,6 +179,7 @@ __global__ void __launch_bounds__(kPgT) kv_reserve_kernel(const KvPool p, const 
     p.ref[id] = 1;
     ++rank;
   }
+  pg_publish();
 }
 
 // One block.  Checks the forks, takes a page for each tail, writes the children's counts and the plan of the copies.
@@ -262,6 +268,7 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(const KvPool p, uint4* kv,
       else atomicOr(&p.ws->status, STATUS_BAD_STREAM);
     }
     if (to >= 0 && threadIdx.x == 0) row[f.z] = to;
+    pg_publish();
     return;
   }
   if (to < 0) return;
@@ -271,6 +278,7 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(const KvPool p, uint4* kv,
   }
   uint4* layer = kv + (blockIdx.x - 1) * layer_units;
   pg_copy(layer + to * block_units, layer + f.w * block_units, units);
+  pg_publish();
 }
 
 // One block.  remap[p]: where used page p lies afterwards (-1: free); the k-th used page behind the first `live` ids takes
@@ -331,6 +339,7 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(const KvPool p, const i
     uint4* layer = kv + i % layers * layer_units;
     pg_copy(layer + m.y * block_units, layer + m.x * block_units, units);
   }
+  pg_publish();
 }
 
 }  // namespace flint

@@ -1162,7 +1162,7 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
                       const float* sinks, int64_t window, float scale, int64_t batch, int64_t tokens, int64_t Hq, void* out,
                       int64_t out_stride, void* ws, int pdl, void* stream) {
   if (!q || !kv || !bt || !seq_lens || !out || !ws) return FLINT_ERR_ARGUMENT;
-  if (window < 0 || window > INT32_MAX || !(scale > 0.f) || !(scale < 1e30f)) return FLINT_ERR_ARGUMENT;
+  if (window < 0 || out == q || !(scale > 0.f) || !(scale < 1e30f)) return FLINT_ERR_ARGUMENT;
   if (batch < 1 || batch > (1 << 20) || tokens < 1 || tokens > (1 << 24) || Hkv < 1 || Hkv > 128 || Hq < 1 || Hq % Hkv != 0 ||
       Hq / Hkv > 8 || num_blocks < 1 || num_blocks >= INT32_MAX || max_blocks < 1 || max_blocks > (1 << 25) || bt_stride < 0 ||
       q_stride < Hq * kPaD || out_stride < Hq * kPaD || stride_head < kPaPage * 2 * kPaD || stride_block < kPaPage * 2 * kPaD)
@@ -1186,7 +1186,8 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   PagedAttnArgs a = {};
   a.block_tables = bt; a.bt_stride = bt_stride; a.max_blocks = (int)max_blocks; a.cu_seqlens = cu_seqlens;
   a.seq_lens = seq_lens; a.group_starts = group_starts; a.prefix_lens = prefix_lens; a.groups = (int)groups; a.sinks = sinks;
-  a.window = (int)window; a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
+  a.window = window >= max_blocks * kPaPage ? 0 : (int)window;    // (a window over every length hides nothing)
+  a.batch = (int)batch; a.tokens = (int)tokens; a.Hkv = (int)Hkv; a.G = G;
   a.num_blocks = (int)num_blocks; a.per = per; a.inv_g = (65536 + G - 1) / G; a.c = scale * kPaLog2e; a.out = (bf16*)out; a.out_stride = out_stride;
   a.wide = aligned(out, 32) && out_stride % 16 == 0;
   a.ws = static_cast<PagedAttnWorkspace*>(ws);

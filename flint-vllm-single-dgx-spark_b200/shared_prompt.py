@@ -57,6 +57,15 @@ class SharedPromptDecoder(Decoder):
         page = self.bt.gather(1, (self.positions // PAGE)[:, None])[:, 0].long()
         self.slots.copy_(torch.where(page >= 0, page * PAGE + self.positions % PAGE, -1))
 
+    def prefill(self, prompts):
+        raise NotImplementedError("SharedPromptDecoder reads one prompt for all streams: read_prompt()")
+
+    def fill_kv_random(self, prompts, seed: int = 0):
+        raise NotImplementedError("the streams' pages come from read_prompt()")
+
+    def generate_host_driven(self, n, pinned):
+        raise NotImplementedError("slots follow the pool's tables on the device: decode()")
+
     # ---- the prompt ----
     @staticmethod
     def _norm(x, res, w, eps):
@@ -133,8 +142,13 @@ class SharedPromptDecoder(Decoder):
         self.check_status()
 
     def branch(self, dst, src):
-        """Streams dst[i] give up their own continuation and go on from where stream src[i] is."""
+        """Streams dst[i] (host ints) give up their own continuation and go on from where stream src[i] is."""
         pool, dev = self.pool, self.m.dev
+        if (len(src) != len(dst) or len(set(dst)) != len(dst) or set(src) & set(dst)
+                or any(not 0 <= b < self.M for b in (*src, *dst))):
+            raise ValueError(f"branch: {dst} from {src} among {self.M} streams")
+        if not dst:
+            return
         src, dst = (torch.as_tensor(v, dtype=torch.int32, device=dev) for v in (src, dst))
         pool.seq_lens.copy_(self.positions)                   # cached tokens; the current one is not yet among them
         pool.free(dst)

@@ -520,7 +520,8 @@ int flint_moe_grouped_down(const void* ah, const int32_t* shift, const int32_t* 
  * query tokens of sequence b are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (none: b is skipped); seq_lens int32 [batch]:
  * the tokens of b in the cache, its queries' own keys included, so query i of n sits at position p = seq_lens[b] - n + i.
  * It sees the keys max(0, p - window + 1) .. p (window 0: all up to p); a query that sees none (p < 0) gives zeros.
- * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written.  Slots of the cache that no
+ * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written; out must not overlap q.  scale is
+ * positive.  Slots of the cache that no
  * query sees may hold anything, NaN and infinities too.  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache
  * 16-byte aligned, strides multiples of 8 elements.  workspace: flint_prefill_attention_workspace_bytes(). */
 int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads);

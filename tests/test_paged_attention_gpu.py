@@ -308,10 +308,13 @@ def test_refusals(fb):
            dict(out=z(5, 8, D)), dict(kv_cache=z(3, 2, 32, 2 * D)), dict(kv_cache=z(3, 2, PAGE, 2 * D, dt=torch.float16)),
            dict(kv_cache=z(3, PAGE, 2, 2 * D).transpose(1, 2)), dict(block_tables=i(2, 3).long()), dict(block_tables=i(1, 3)),
            dict(cu_seqlens=i(2)), dict(seq_lens=i(2).long()), dict(sinks=z(8)), dict(sinks=z(7, dt=torch.float32)),
-           dict(window=-1), dict(cu_seqlens=i(3).cpu()), dict(seq_lens=i(2).cpu())]
+           dict(window=-1), dict(out=None), dict(cu_seqlens=i(3).cpu()), dict(seq_lens=i(2).cpu())]
     for change in bad:
+        args = {**good, **change}
+        if args["out"] is None:
+            args["out"] = args["q"]                               # in place
         with pytest.raises(fb._lib.FlintError):
-            pa.flint_prefill_attention(**{**good, **change})
+            pa.flint_prefill_attention(**args)
     good = dict(q=z(2, 8, D), kv_cache=z(3, 2, PAGE, 2 * D), block_tables=i(2, 3), seq_lens=i(2),
                 group_starts=torch.tensor([0, 2], dtype=torch.int32, device="cuda"), prefix_lens=i(1), sinks=None, window=None,
                 scale=SCALE, out=z(2, 8, D))
@@ -322,6 +325,22 @@ def test_refusals(fb):
             sp.flint_shared_prefix_attention(**{**good, **change})
     torch.cuda.synchronize()
     fb._lib.device_status(clear=True)
+
+
+def test_registered_ops_and_widest_window(fb):
+    """torch.ops gives the shim's bits; a window wider than any length is no window; out may lie at 16 bytes."""
+    from flint_b200 import prefill_attention as pa
+    args, out = run_prefill(np.random.default_rng(20), [40, 70], [40, 300], 2, 4, 0, True)
+    first = host(out).copy()
+    torch.ops.flint_b200.prefill_attention(*args[:6], 0, SCALE, out.zero_())
+    np.testing.assert_array_equal(host(out), first)
+    for window in (2 ** 31 - 1, 2 ** 40, 16 * args[2].shape[1]):
+        pa.flint_prefill_attention(*args[:6], window, SCALE, out.zero_())
+        np.testing.assert_array_equal(host(out), first)
+    odd = torch.zeros(out.numel() + 8, dtype=torch.bfloat16, device="cuda")[8:].view(out.shape)
+    assert odd.data_ptr() % 32 == 16
+    pa.flint_prefill_attention(*args[:8], odd)
+    np.testing.assert_array_equal(host(odd), first)
 
 
 def test_no_rows(fb):

@@ -49,13 +49,13 @@ def test_fake_tensors_reach_the_registered_ops(fb):
 
 P = ctypes.c_void_p(256)
 PREFILL = dict(q=P, q_stride=4096, kv=P, blocks=8, Hkv=4, sb=16384, sh=4096, bt=P, bts=4, max_blocks=4, cu=P, lens=P,
-               sinks=None, window=0, scale=0.1, batch=2, tokens=9, Hq=32, out=P, out_stride=4096, ws=P, pdl=0, stream=None)
+               sinks=None, window=0, scale=0.1, batch=2, tokens=9, Hq=32, out=ctypes.c_void_p(512), out_stride=4096, ws=P, pdl=0, stream=None)
 ARGUMENT, SHAPE, ALIGN = 6, 1, 2
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(q=None), ARGUMENT), (dict(kv=None), ARGUMENT), (dict(cu=None), ARGUMENT), (dict(lens=None), ARGUMENT),
-    (dict(ws=None), ARGUMENT), (dict(window=-1), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-0.1), ARGUMENT),
+    (dict(ws=None), ARGUMENT), (dict(window=-1), ARGUMENT), (dict(out=P, q=P), ARGUMENT), (dict(scale=0.0), ARGUMENT), (dict(scale=-0.1), ARGUMENT),
     (dict(scale=float("nan")), ARGUMENT), (dict(scale=float("inf")), ARGUMENT), (dict(batch=0), SHAPE),
     (dict(tokens=0), SHAPE), (dict(tokens=1 << 25), SHAPE), (dict(Hq=30), SHAPE), (dict(Hq=36), SHAPE), (dict(Hkv=0), SHAPE),
     (dict(blocks=0), SHAPE), (dict(max_blocks=0), SHAPE), (dict(max_blocks=1 << 26), SHAPE), (dict(q_stride=4088), SHAPE),
@@ -68,7 +68,7 @@ def test_prefill_arguments_are_checked_on_the_host(fb, change, code):
 
 def test_shared_prefix_groups_are_checked_on_the_host(fb):
     L = fb._lib.lib()
-    args = [P, 4096, P, 8, 4, 16384, 4096, P, 4, 4, P, P, P, 1, None, 0, 0.1, 2, 32, P, 4096, P, 0, None]
+    args = [P, 4096, P, 8, 4, 16384, 4096, P, 4, 4, P, P, P, 1, None, 0, 0.1, 2, 32, ctypes.c_void_p(512), 4096, P, 0, None]
     for at, value, code in ((11, None, ARGUMENT), (12, None, ARGUMENT), (13, 0, SHAPE), (13, 3, SHAPE), (17, 0, SHAPE)):
         assert L.flint_shared_prefix_attention(*[value if i == at else v for i, v in enumerate(args)]) == code
 

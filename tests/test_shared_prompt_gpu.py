@@ -130,4 +130,13 @@ def test_refusals(fb):
         dec.read_prompt(np.zeros(150, np.int64), room=40)
     with pytest.raises(ValueError):
         dec.read_prompt(np.zeros(0, np.int64), room=4)
+    dec.read_prompt(np.zeros(20, np.int64), room=4)
+    for dst, src in (([1], [1]), ([0, 1], [1, 0]), ([2], [0]), ([0], []), ([1, 1], [0, 0])):
+        with pytest.raises(ValueError):
+            dec.branch(dst, src)
+    dec.branch([], [])
+    for call in (lambda: dec.prefill(np.zeros((2, 4), np.int64)), lambda: dec.fill_kv_random(np.zeros((2, 4))),
+                 lambda: dec.generate_host_driven(1, {})):
+        with pytest.raises(NotImplementedError):
+            call()
     dec.close()
