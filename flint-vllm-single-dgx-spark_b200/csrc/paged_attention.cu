@@ -10,7 +10,7 @@
 //
 // Work.  An item is one KV head and up to two row tiles of 128 rows: floor(128 / G) consecutive query tokens (or streams)
 // with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys and
-// a constant, for one tile as for two), the line is cut into equal shares, one per SM: a long prompt's items and a few
+// a constant), the line is cut into equal shares, one per SM: a long prompt's items and a few
 // rows on a long cache are both split evenly, and where a cut falls into an item its parts leave (m, l, o) in the
 // workspace and a second launch joins them in the order of the keys.
 //   an item of two tiles: both tiles multiply the same keys; one's softmax runs under the other's products
@@ -51,7 +51,8 @@ constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA,
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaFixed = 225;                  // cost of an item beside its keys, in keys (128 keys take some 1.9 us)
+constexpr int kPaFixed2 = 260, kPaFixed1 = 120;  // cost of an item of two tiles / of one beside its keys, in keys (128
+                                               // keys take some 2 us; an item 4 or 2 us more)
 constexpr int kPaLeast = 200;                  // least share of a block, in keys
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4;
@@ -386,6 +387,7 @@ struct PaLine {
     }
     return s.ntok <= tile ? (n + kPaKeys - 1) & ~(kPaKeys - 1) : n;
   }
+  __device__ int fixed(const PaSegment& s, int i) const { return tokens_of(s, i) > per ? kPaFixed2 : kPaFixed1; }
   // cost of the items before item k
   __device__ long long upto(const PaSegment& s, int k) const {
     const int m = (s.ntok + tile - 1) / tile;
@@ -397,11 +399,11 @@ struct PaLine {
       w = pa_ramp(s.pos0 + tile, tile, whole);
       if (a.window > 0) w -= pa_ramp(s.pos0 - a.window + 1, tile, whole);
     }
-    if (k >= m) w += keys(s, m - 1);
-    return w + (long long)kPaFixed * min(k, m);
+    if (k >= m) w += keys(s, m - 1) + fixed(s, m - 1);
+    return w + (long long)kPaFixed2 * whole;
   }
 };
-static_assert(kPaFixed > 0, "every item has a place on the line");
+static_assert(kPaFixed1 > 0 && kPaFixed2 > 0, "every item has a place on the line");
 
 __global__ void __launch_bounds__(kPaThreads, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const PagedAttnArgs a) {
@@ -545,11 +547,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
           }
         }
         long long start = seg0 + h * s.cost + line.upto(s, i);
-        int w = 0;
+        int w = 0, fixed = 0;
         for (; h < a.Hkv && ok && start < x1; ++h, i = 0)
-          for (; i < m && start < x1; ++i, start += kPaFixed + w) {
-            w = line.keys(s, i);
-            const long long stop = start + kPaFixed + w;
+          for (; i < m && start < x1; ++i, start += fixed + w) {
+            w = line.keys(s, i), fixed = line.fixed(s, i);
+            const long long stop = start + fixed + w;
             PaItem it;
             it.tok0 = s.tok0 + i * line.tile, it.ntok = line.tokens_of(s, i), it.h = h, it.table = s.table;
             it.dual = it.ntok > line.per;
@@ -577,7 +579,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             const unsigned unit = steps ? max(1u, ((unsigned)w + steps - 1) / (unsigned)steps) : 1u;
             auto before = [&](long long x) -> int {
               if (x >= stop) return steps;
-              return x <= start + kPaFixed ? 0 : min(steps, (int)((unsigned)(x - start - kPaFixed) / unit));
+              return x <= start + fixed ? 0 : min(steps, (int)((unsigned)(x - start - fixed) / unit));
             };
             it.j0 = before(x0), it.j1 = before(x1);
             PaRecord rec = {PA_NONE, PA_NONE, it.tok0, !s.home && s.lo > 0};
