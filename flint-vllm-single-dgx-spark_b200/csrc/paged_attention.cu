@@ -9,21 +9,29 @@
 // 2^(sink log2 e - c m) to l.  A row without keys gives zeros.
 //
 // Work.  An item is one KV head and up to two row tiles of 128 rows: floor(128 / G) consecutive query tokens (or streams)
-// with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys and
-// a constant), the line is cut into equal shares, one per SM: a long prompt's items and a few
-// rows on a long cache are both split evenly, and where a cut falls into an item its parts leave (m, l, o) in the
-// workspace and a second launch joins them in the order of the keys.
+// with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys and a
+// constant) and the line is cut into equal shares, one per SM: a long prompt's items and a few rows on a long cache are both
+// split evenly.  Where a cut falls into an item its parts leave (m, l, o) in the workspace, and a second launch joins them in
+// the order of the keys, so results repeat bit for bit.
 //   an item of two tiles: both tiles multiply the same keys; one's softmax runs under the other's products
 //   an item of one tile:  its keys are dealt to the two halves of the block in turn, and joined at the end
 //
 // Block: two softmax groups of 4 warps (a thread per row), a warp each for TMA, for the MMAs and for cutting the items.
 // Keys come 128 at a time: 8 pages, one TMA box of 16 tokens x 64 columns per half of K or V, 128-byte swizzle, into a ring
 // of four 32 KB slots.  S = Q K^T (both from shared memory) and O += P V (P from tensor memory, where it overwrites its S;
-// V as it lies, tokens as the K dimension) are tcgen05 products of 128 x 128 x 128, issued by one lane.  The MMAs of one
-// thread run in order, so when S of a step has come, the O of the step before is complete: the softmax group may rescale
+// V as it lies, tokens as the K dimension) are tcgen05 products of 128 x 128 x 128, issued by one elected lane.  The MMAs of
+// one thread run in order, so when S of a step has come, the O of the step before is complete: the softmax group may rescale
 // it.  It does so only when a row's maximum rises by more than 2^8 over the reference, which the first steps do.
 // Slots that no row may see are never multiplied: a page that an item does not reach is read out of bounds (zeros), and
 // its last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too.
+//
+// Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 290 us (1.04 PFLOP/s), of 16,421 tokens 1.85 ms (1.19), in long
+// runs at the card's power limit 327 us and 2.11 ms; 192 streams on three prefixes of up to 16,384 tokens 109 us.  A step of
+// two tiles, 2,048 cycles of products, takes some 1.9 us: the tensor pipe is busy for 52 to 62% of it, the rest is the way
+// S -> softmax (1.4 us) -> P -> S through four barriers.  Without the maximum or without the exponentials a prompt is only 6%
+// faster; two threads a row (16 softmax warps) cost 20%, S in two buffers of 64 keys 5% (an MMA of N = 64 takes as long as
+// one of N = 128), a share of the exponentials on the FMA pipes nothing.  What a call costs besides: 5 us to its first item
+// and 3 us for the join's launch, which bound the small ones; an item, 2 to 4 us of filling and draining.
 #include <limits.h>
 
 #include <atomic>
@@ -51,8 +59,9 @@ constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA,
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaFixed2 = 260, kPaFixed1 = 120;  // cost of an item of two tiles / of one beside its keys, in keys (128
-                                               // keys take some 2 us; an item 4 or 2 us more)
+constexpr int kPaFixed2 = 260, kPaFixed1 = 120;  // cost of an item of two tiles / of one beside its keys, in keys (a step
+                                               // of 128 takes some 2 us, an item 4 or 2 us more; with 225 for both
+                                               // 192 streams took 114 us, with these 109)
 constexpr int kPaLeast = 200;                  // least share of a block, in keys
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4;
@@ -476,6 +485,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
     if (lane == 0) runs[i0 / 32] = c;
   }
+  fence_proxy_async();                                            // (TMA writes these bytes later)
   __syncthreads();
 
   if (warp == 10) {
@@ -617,6 +627,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
               ok = false;
               break;
             }
+            if (n_items == 0) fence_proxy_async();                // the ring's bytes have been read
             if (lane == 0) {
               items[q] = it;
               mbar_arrive(&b_item[q]);
