@@ -276,6 +276,9 @@ __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
 }
 
 // A wait for the phase of the given parity that gives up after two seconds, or as soon as another warp of the block has.
+// The lanes of a warp may not agree on that: what the whole warp has to do alike depends on a vote (pa_all).  The warps of
+// the products and of the softmax vote once a step and go on until then (a vote behind each wait: 294 us against 281 for
+// 6,057 tokens).
 constexpr unsigned long long kPaWaitNs = 2000000000ull;
 __device__ __forceinline__ unsigned long long pa_now() {
   unsigned long long t;
@@ -299,6 +302,13 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, unsigned parity, volatile
   for (int i = 0; i < 32; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return pa_wait_long(bar, parity, failed, status);
+}
+__device__ __forceinline__ bool pa_all(bool ok) { return __all_sync(0xffffffffu, ok); }
+// The same after a wait has run out, for copies and products that are still in flight.
+__device__ __noinline__ void pa_drain(uint64_t* bar, unsigned parity) {
+  const unsigned long long t0 = pa_now();
+  while (!mbar_try_wait(bar, parity) && pa_now() - t0 < kPaWaitNs) {
+  }
 }
 
 // row / G of a row below 256 (exact: the error of inv_g is below 1 / 256 of a quotient's step)
@@ -426,10 +436,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   float4* sx = reinterpret_cast<float4*>(ring + kPaSlots * kPaSlotBytes);   // 32 columns of o between the halves
   __shared__ PaItem items[kPaQueue];
   __shared__ __align__(8) uint64_t b_item[kPaQueue], b_item_free[kPaQueue], b_full[kPaSlots], b_empty[kPaSlots], b_q, b_q_free,
-      b_s[2], b_p[4], b_o[2], b_hand, b_take;
+      b_s[2], b_p[4], b_o[2], b_hand, b_take, b_end;
   __shared__ float2 s_ml[kPaM];
   __shared__ uint32_t s_taddr;
   __shared__ int s_failed;                                        // a wait ran out: every warp leaves
+  __shared__ int s_sent[2];                                       // copies that were started: of keys, of Q
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned* status = &a.ws->status;
   if (tid == 0) {
@@ -447,6 +458,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     mbar_init(&b_q_free, 1);
     mbar_init(&b_hand, 4);
     mbar_init(&b_take, 4);
+    mbar_init(&b_end, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b_s[t], 1);
       mbar_init(&b_p[2 * t], 4);                                  // P of the last 112 and of the first 16 keys
@@ -627,7 +639,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
               cut_item = {rec.first, rec.last, it.tok0, it.ntok, h};
             }
             const int q = n_items % kPaQueue;
-            if (n_items >= kPaQueue && !pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status)) {
+            if (n_items >= kPaQueue && !pa_all(pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status))) {
               ok = false;
               break;
             }
@@ -646,7 +658,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     if (lane == 0 && !line.shared) a.split[blockIdx.x] = cut_item;
     // an item without tokens ends the block
     const int q = n_items % kPaQueue;
-    if (n_items >= kPaQueue && ok) ok = pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status);
+    if (n_items >= kPaQueue && ok) ok = pa_all(pa_wait(&b_item_free[q], (unsigned)((n_items / kPaQueue - 1) & 1), &s_failed, status));
     if (ok && lane == 0) {
       items[q].ntok = 0;
       mbar_arrive(&b_item[q]);
@@ -654,10 +666,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     __syncwarp();
   } else if (warp == 8) {
     // ---- TMA ----
-    int slot = 0, parity = 1, nq = 0;                             // an empty ring's slots count as released
+    int slot = 0, parity = 1, nq = 0, sent = 0, q_sent = 0;       // an empty ring's slots count as released
     bool ok = true;
-    for (int n = 0; ok; ++n) {
-      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+    for (int n = 0; pa_all(ok); ++n) {
+      if (!pa_all(pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status))) break;
       const PaItem it = items[n % kPaQueue];
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
@@ -678,48 +690,47 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         }
         const int blk = __shfl_sync(0xffffffffu, ids, (j & 3) * 8 + (lane & 7));
         if (ok && !pa_wait(&b_empty[slot], (unsigned)parity, &s_failed, status)) ok = false;
-        if (ok) {
-          if (lane == 0) mbar_arrive_expect_tx(&b_full[slot], kPaSlotBytes);
-          __syncwarp();
-          if (lane < 8) {
-            const int left = it.end - (p0 + lane) * kPaPage;      // tokens from this page on
-            const int shift = left > 0 && left < kPaPage ? kPaPage - left : 0;
-            const uint32_t dst = smem_u32(ring + slot * kPaSlotBytes) + lane * kPaPageHalf;
-            pa_tma_4d(dst, &mkv, column, -shift, it.h, blk, &b_full[slot]);
-            pa_tma_4d(dst + kPaHalf, &mkv, column + 64, -shift, it.h, blk, &b_full[slot]);
-          }
-          __syncwarp();
+        if (ok && lane == 0) mbar_arrive_expect_tx(&b_full[slot], kPaSlotBytes);
+        sent += ok;
+        __syncwarp();
+        if (ok && lane < 8) {
+          const int left = it.end - (p0 + lane) * kPaPage;        // tokens from this page on
+          const int shift = left > 0 && left < kPaPage ? kPaPage - left : 0;
+          const uint32_t dst = smem_u32(ring + slot * kPaSlotBytes) + lane * kPaPageHalf;
+          pa_tma_4d(dst, &mkv, column, -shift, it.h, blk, &b_full[slot]);
+          pa_tma_4d(dst + kPaHalf, &mkv, column + 64, -shift, it.h, blk, &b_full[slot]);
         }
+        __syncwarp();
         if (++slot == kPaSlots) slot = 0, parity ^= 1;
       };
-      // Q as soon as its buffer is free; the keys need not wait for that
-      const bool early = mbar_try_wait(&b_q_free, (unsigned)((nq & 1) ^ 1));
-      if (!early) load(it.j0, 0);
-      if (ok && !pa_wait(&b_q_free, (unsigned)((nq & 1) ^ 1), &s_failed, status)) ok = false;
-      ++nq;
-      if (ok && lane == 0) {
-        const int tiles = it.dual ? 2 : 1, per = a.per;
-        mbar_arrive_expect_tx(&b_q, (unsigned)(tiles * 2 * per * a.G * 128));
-        for (int t = 0; t < tiles; ++t)
-          for (int half = 0; half < 2; ++half)
-            pa_tma_3d(smem_u32(sq) + t * kPaSlotBytes + half * kPaHalf, &mq, half * 64, it.h * a.G, it.tok0 + t * per, &b_q);
-      }
-      __syncwarp();
-      if (early) load(it.j0, 0);
-      if (n == 0 && lane == 0) FLINT_TL(5);
-      if (it.dual) {                                              // K0 V0 K1 V1 ..
-        for (int j = it.j0; j < it.j1; ++j) {
-          if (j > it.j0) load(j, 0);
-          load(j, 128);
+      // Q as soon as its buffer is free; the first keys need not wait for that.  One copy of this code: a call of one step
+      // takes as long as its instructions take to come.
+      const int q_at = __all_sync(0xffffffffu, mbar_try_wait(&b_q_free, (unsigned)((nq & 1) ^ 1))) ? 0 : 1;
+      int kj = it.j0, vj = it.j0;                                 // the next step of K, of V
+#pragma unroll 1
+      for (int i = 0; vj < it.j1; ++i) {
+        if (i == q_at) {
+          if (ok && !pa_wait(&b_q_free, (unsigned)((nq & 1) ^ 1), &s_failed, status)) ok = false;
+          if (ok && lane == 0) {
+            const int tiles = it.dual ? 2 : 1, per = a.per;
+            mbar_arrive_expect_tx(&b_q, (unsigned)(tiles * 2 * per * a.G * 128));
+#pragma unroll 1
+            for (int t = 0; t < 2 * tiles; ++t)
+              pa_tma_3d(smem_u32(sq) + t * kPaHalf, &mq, (t & 1) * 64, it.h * a.G, it.tok0 + (t >> 1) * per, &b_q);
+          }
+          q_sent += ok;
+          ++nq;
+          __syncwarp();
         }
-      } else {                                                    // K0 K1 V0 K2 V1 K3 ..
-        if (steps > 1) load(it.j0 + 1, 0);
-        for (int j = it.j0; j < it.j1; ++j) {
-          load(j, 128);
-          if (j + 2 < it.j1) load(j + 2, 0);
-        }
+        // two tiles: K0 V0 K1 V1 ..; one: K0 K1 V0 K2 V1 ..
+        const bool k = kj < it.j1 && kj - vj < (it.dual ? 1 : 2);
+        load(k ? kj : vj, k ? 0 : 128);
+        if (k) ++kj;
+        else ++vj;
+        if (n == 0 && i == 0 && lane == 0) FLINT_TL(5);
       }
     }
+    if (lane == 0) s_sent[0] = sent, s_sent[1] = q_sent;
   } else if (warp == 9) {
     // ---- MMA ----
     int slot = 0, parity = 0, p_par[2] = {0, 0}, nq = 0;
@@ -730,7 +741,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     constexpr uint32_t kTile = kPaSlotBytes >> 4;
     auto next = [&]() {                                           // the next slot of the ring, filled
       const int at = slot;
-      if (ok && !pa_wait(&b_full[at], (unsigned)parity, &s_failed, status)) ok = false;
+      ok &= pa_wait(&b_full[at], (unsigned)parity, &s_failed, status);
       if (++slot == kPaSlots) slot = 0, parity ^= 1;
       return at;
     };
@@ -741,15 +752,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     auto pv = [&](int t, int v, bool add) {                       // O += P V, in two parts as P comes
 #pragma unroll
       for (int part = 0; part < 2; ++part) {
-        if (ok && !pa_wait(&b_p[2 * t + part], (unsigned)p_par[t], &s_failed, status)) ok = false;
-        if (!ok) return;
+        ok &= pa_wait(&b_p[2 * t + part], (unsigned)p_par[t], &s_failed, status);
         pa_fence_after();
         pa_mma_pv(base + 256 + 128 * t, base + 128 * t + 64, v_desc + v * kTile, part, add);
       }
       p_par[t] ^= 1;
     };
-    for (int n = 0; ok; ++n) {
-      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+    for (int n = 0;; ++n) {
+      if (!pa_all(ok && pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status))) break;
       const PaItem& it = items[n % kPaQueue];
       const int ntok = __shfl_sync(0xffffffffu, it.ntok, 0), dual = __shfl_sync(0xffffffffu, it.dual, 0),
                 steps = __shfl_sync(0xffffffffu, it.j1 - it.j0, 0);
@@ -757,28 +767,25 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       __syncwarp();
       if (ntok == 0) break;
       if (steps == 0) continue;
-      if (!pa_wait(&b_q, (unsigned)(nq++ & 1), &s_failed, status)) break;
+      ok &= pa_wait(&b_q, (unsigned)(nq++ & 1), &s_failed, status);
       if (n == 0 && lane == 0) FLINT_TL(6);
       pa_fence_after();
       if (dual) {
         int k = next();
-        if (!ok) break;
         qk(0, 0, k);
         qk(1, 1, k);
         pa_commit(&b_empty[k]);
         if (steps == 1) pa_commit(&b_q_free);
-        for (int j = 0; j < steps && ok; ++j) {
+        for (int j = 0; j < steps && pa_all(ok); ++j) {
           const int v = next();
           if (j + 1 < steps) k = next();
           pv(0, v, j > 0);
-          if (!ok) break;
           if (j + 1 < steps) {
             qk(0, 0, k);
           } else {
             pa_commit(&b_o[0]);
           }
           pv(1, v, j > 0);
-          if (!ok) break;
           pa_commit(&b_empty[v]);
           if (j + 1 < steps) {
             qk(1, 1, k);
@@ -791,20 +798,17 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       } else {
         for (int t = 0; t < 2 && t < steps; ++t) {
           const int k = next();
-          if (!ok) break;
           qk(t, 0, k);
           pa_commit(&b_empty[k]);
           if (t + 1 == steps) pa_commit(&b_q_free);
         }
-        for (int j = 0; j < steps && ok; ++j) {
+        for (int j = 0; j < steps && pa_all(ok); ++j) {
           const int t = j & 1, v = next();
           if (t) pv(1, v, j > 1);
           else pv(0, v, j > 1);
-          if (!ok) break;
           pa_commit(&b_empty[v]);
           if (j + 2 < steps) {
             const int k = next();
-            if (!ok) break;
             qk(t, 0, k);
             pa_commit(&b_empty[k]);
             if (j + 3 == steps) pa_commit(&b_q_free);
@@ -821,8 +825,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
     const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
     int s_par = 0, o_par = 0, handed = 0;                         // handed: quarters of o from group 1 to group 0 so far
     bool ok = true;
-    for (int n = 0; ok; ++n) {
-      if (!pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status)) break;
+    for (int n = 0;; ++n) {
+      if (!pa_all(pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status))) break;
       const PaItem it = items[n % kPaQueue];
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
@@ -843,11 +847,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       const int stride = it.dual ? 1 : 2, mine0 = it.dual ? 0 : t;
       const int last_page = it.end & ~(kPaPage - 1);              // a cut last page: its tokens lie at its slot's end
       const int shift = it.end > last_page ? kPaPage - (it.end - last_page) : 0;
-      for (int j = mine0; j < steps && ok; j += stride) {
-        if (!pa_wait(&b_s[t], (unsigned)s_par, &s_failed, status)) {
-          ok = false;
-          break;
-        }
+      for (int j = mine0; j < steps && pa_all(ok); j += stride) {
+        ok &= pa_wait(&b_s[t], (unsigned)s_par, &s_failed, status);
         s_par ^= 1;
         pa_fence_after();
         if (n == 0 && j == 0 && tid == 0) FLINT_TL(7);
@@ -950,18 +951,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         if (n == 0 && j == 0 && tid == 0) FLINT_TL(8);
       }
       const bool any = mine0 < steps;
-      if (any && ok) {
-        if (!pa_wait(&b_o[t], (unsigned)o_par, &s_failed, status)) ok = false;
+      if (any) {
+        ok &= pa_wait(&b_o[t], (unsigned)o_par, &s_failed, status);
         o_par ^= 1;
         pa_fence_after();
         if (n == 0 && tid == 0) FLINT_TL(9);
       }
-      if (!ok) break;
+      if (!pa_all(ok)) break;
       // two halves of one tile: group 1 hands its (m, l, o) over, 64 columns at a time
       const bool join = !it.dual && steps > 1;
       float f0 = 1.f, f1 = 0.f;
       auto hand = [&](const uint32_t* o, int quarter) {           // group 1: 32 columns (and m, l beside the first ones)
-        if (handed > 0 && !pa_wait(&b_take, (unsigned)((handed - 1) & 1), &s_failed, status)) ok = false;
+        if (handed > 0) ok &= pa_wait(&b_take, (unsigned)((handed - 1) & 1), &s_failed, status);
         if (quarter == 0) s_ml[row] = make_float2(m, l);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -972,7 +973,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         ++handed;
       };
       auto take = [&](uint32_t* o, int quarter) {                 // group 0
-        if (ok && !pa_wait(&b_hand, (unsigned)(handed & 1), &s_failed, status)) ok = false;
+        ok &= pa_wait(&b_hand, (unsigned)(handed & 1), &s_failed, status);
         if (quarter == 0) {
           const float2 other = s_ml[row];
           const float mm = fmaxf(m, other.x);
@@ -1048,6 +1049,16 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   }
   pa_fence_before();
   __syncthreads();
+  if (s_failed) {                                                 // nothing may be in flight when the block's memory goes
+    if (warp == 8) {
+      for (int k = max(0, s_sent[0] - kPaSlots); k < s_sent[0]; ++k) pa_drain(&b_full[k % kPaSlots], (unsigned)(k / kPaSlots & 1));
+      if (s_sent[1]) pa_drain(&b_q, (unsigned)(s_sent[1] - 1 & 1));
+    } else if (warp == 9) {
+      pa_commit(&b_end);
+      pa_drain(&b_end, 0);
+    }
+    __syncthreads();
+  }
   if (tid == 0) FLINT_TL(11);
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kPaTmem) : "memory");
