@@ -22,8 +22,9 @@
 // V as it lies, tokens as the K dimension) are tcgen05 products of 128 x 128 x 128, issued by one elected lane.  The MMAs of
 // one thread run in order, so when S of a step has come, the O of the step before is complete: the softmax group may rescale
 // it.  It does so only when a row's maximum rises by more than 2^8 over the reference, which the first steps do.
-// Slots that no row may see are never multiplied: a page that an item does not reach is read out of bounds (zeros), and
-// its last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too.
+// Slots that no row may see are never multiplied: a page that an item does not reach is read out of bounds (zeros), its
+// last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too, and rows
+// of V that a window has left behind in the first page are cleared in shared memory.
 //
 // Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 290 us (1.04 PFLOP/s), of 16,421 tokens 1.85 ms (1.19), in long
 // runs at the card's power limit 327 us and 2.11 ms; 192 streams on three prefixes of up to 16,384 tokens 109 us.  A step of
@@ -111,6 +112,7 @@ struct PaItem {
   int j0, j1;                                  // steps of this part
   int pos0;                                    // position of the first token; prefix: -1
   int dual;
+  int dead;                                    // rows of the first page's slot whose keys no row of the item sees
   int out;                                     // slot, PA_HOME or PA_FINAL
   int home;                                    // 0: own keys, 1: prefix
 };
@@ -582,23 +584,28 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
             it.dual = it.ntok > line.per;
             it.home = s.home;
             if (s.home) {                                         // the keys that the tile's streams see of the prefix
-              int lo = INT_MAX, hi = 0;
+              int lo = INT_MAX, hi = 0, by = 0;
               for (int r = lane; r < it.ntok; r += 32) {
                 const int len = line.length(it.tok0 + r);
-                hi = max(hi, len);
+                if (len > hi) hi = len, by = it.tok0 + r;
                 if (len > 0) lo = min(lo, a.window > 0 ? max(0, len - a.window) : 0);
               }
-              hi = __reduce_max_sync(0xffffffffu, hi);
+              const int most = __reduce_max_sync(0xffffffffu, hi);  // that stream's table has every page that one of them sees
+              it.table = __reduce_min_sync(0xffffffffu, hi == most ? by : INT_MAX);
+              hi = most;
               lo = __reduce_min_sync(0xffffffffu, lo);
               it.pos0 = -1;
               it.end = min(s.hi, hi);
               it.begin = lo < it.end ? lo & ~(kPaPage - 1) : it.end;
+              it.dead = lo < it.end ? lo - it.begin : 0;
             } else {
               it.pos0 = s.pos0 + i * line.tile;
               it.end = max(0, it.pos0 + it.ntok);
-              it.begin = max(s.lo, a.window > 0 ? max(0, it.pos0 - a.window + 1) & ~(kPaPage - 1) : 0);
-              if (it.begin > it.end) it.begin = it.end;
+              const int lo = a.window > 0 ? max(0, it.pos0 - a.window + 1) : 0;
+              it.begin = min(max(s.lo, lo & ~(kPaPage - 1)), it.end);
+              it.dead = max(0, lo - it.begin);
             }
+            if (it.dead > 0 && it.end < it.begin + kPaPage) it.dead += it.begin + kPaPage - it.end;   // the last page too
             const int steps = (it.end - it.begin + kPaKeys - 1) / kPaKeys;
             // how many steps lie before place x of the line
             const unsigned unit = steps ? max(1u, ((unsigned)w + steps - 1) / (unsigned)steps) : 1u;
@@ -758,11 +765,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       }
       p_par[t] ^= 1;
     };
+    // what a window has left behind may be anything, and 0 times NaN is NaN
+    auto clear = [&](int v, int rows) {
+      for (int i = lane; i < rows * 16; i += 32)
+        *reinterpret_cast<uint4*>(ring + v * kPaSlotBytes + (i & 1) * kPaHalf + (i >> 1) * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async();
+      __syncwarp();
+    };
     for (int n = 0;; ++n) {
       if (!pa_all(ok && pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status))) break;
       const PaItem& it = items[n % kPaQueue];
       const int ntok = __shfl_sync(0xffffffffu, it.ntok, 0), dual = __shfl_sync(0xffffffffu, it.dual, 0),
-                steps = __shfl_sync(0xffffffffu, it.j1 - it.j0, 0);
+                steps = __shfl_sync(0xffffffffu, it.j1 - it.j0, 0), dead = __shfl_sync(0xffffffffu, it.j0 ? 0 : it.dead, 0);
       if (lane == 0) mbar_arrive(&b_item_free[n % kPaQueue]);
       __syncwarp();
       if (ntok == 0) break;
@@ -779,6 +793,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         for (int j = 0; j < steps && pa_all(ok); ++j) {
           const int v = next();
           if (j + 1 < steps) k = next();
+          if (j == 0 && dead > 0) clear(v, dead);
           pv(0, v, j > 0);
           if (j + 1 < steps) {
             qk(0, 0, k);
@@ -804,6 +819,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         }
         for (int j = 0; j < steps && pa_all(ok); ++j) {
           const int t = j & 1, v = next();
+          if (j == 0 && dead > 0) clear(v, dead);
           if (t) pv(1, v, j > 1);
           else pv(0, v, j > 1);
           pa_commit(&b_empty[v]);

@@ -294,6 +294,58 @@ def test_shared_bad_groups_are_reported(fb):
             fb._lib.check_device_status()
 
 
+# ---- what no query sees ----
+def forget(kv, bt, dead):
+    """NaN in the first dead[b] tokens of stream b."""
+    bt = bt.cpu()
+    for b, n in enumerate(dead):
+        for j in range(max(0, n)):
+            kv[int(bt[b, j // PAGE]), :, j % PAGE] = float("nan")
+
+
+@pytest.mark.parametrize("window", [1, 3, 5, 37, 100, 131, 300])
+@pytest.mark.parametrize("q_lens,lens", [([1, 20, 3, 1, 2], [700, 140, 33, 10, 16]), ([300], [900]), ([1], [5000])])
+def test_prefill_window_leaves_anything_behind(fb, window, q_lens, lens):
+    from flint_b200 import prefill_attention as pa
+    args, out = run_prefill(np.random.default_rng(window + len(lens)), q_lens, lens, 2, 4, window, True)
+    was = host(out).copy()
+    forget(args[1], args[2], [n - q - window + 1 for q, n in zip(q_lens, lens)])
+    out.zero_()
+    pa.flint_prefill_attention(*args)
+    np.testing.assert_array_equal(host(out), was)
+
+
+@pytest.mark.parametrize("window", [1, 6, 40, 100, 250])
+@pytest.mark.parametrize("groups,prefix,lens", [([3, 2], [512, 64], [513, 530, 521, 75, 190]), ([40], [2048], list(range(2050, 2090))),
+                                                ([1, 1], [0, 0], [10, 300])])
+def test_shared_window_leaves_anything_behind(fb, window, groups, prefix, lens):
+    from flint_b200 import shared_prefix_attention as sp
+    args, out = run_shared(np.random.default_rng(window + len(lens)), groups, prefix, lens, 2, 4, window, False)
+    was = host(out).copy()
+    dead, at = [], 0
+    for n, p in zip(groups, prefix):
+        first = min(lens[at:at + n]) - window                     # of the shared pages, what the group's shortest stream sees
+        dead += [min(first, p) if lens[b] - window < p else lens[b] - window if first >= p else 0 for b in range(at, at + n)]
+        at += n
+    forget(args[1], args[2], dead)
+    out.zero_()
+    sp.flint_shared_prefix_attention(*args)
+    np.testing.assert_array_equal(host(out), was)
+
+
+@pytest.mark.parametrize("lens", [[0, 300, 17, 290], [40, 0, 0, 261], [256, 255, 270, 0]])
+def test_shared_tables_end_with_their_streams(fb, lens):
+    """Padded and short streams, first in their group too, whose tables do not name the whole prefix."""
+    from flint_b200 import shared_prefix_attention as sp
+    args, out = run_shared(np.random.default_rng(21), [4], [256], lens, 2, 8, 0, True)
+    was = host(out).copy()
+    for b, n in enumerate(lens):
+        args[2][b, -(-n // PAGE):] = -1
+    out.zero_()
+    sp.flint_shared_prefix_attention(*args)
+    np.testing.assert_array_equal(host(out), was)
+
+
 # ---- refusals on the host ----
 def test_refusals(fb):
     from flint_b200 import prefill_attention as pa
