@@ -26,13 +26,13 @@
 // last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too, and rows
 // of V that a window has left behind in the first page are cleared in shared memory.
 //
-// Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 290 us (1.04 PFLOP/s), of 16,421 tokens 1.85 ms (1.19), in long
-// runs at the card's power limit 327 us and 2.11 ms; 192 streams on three prefixes of up to 16,384 tokens 109 us.  A step of
+// Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 283 us (1.06 PFLOP/s), of 16,421 tokens 1.8 ms (1.2), in long
+// runs at the card's power limit 325 us and 2.11 ms; 192 streams on three prefixes of up to 16,384 tokens 101 us.  A step of
 // two tiles, 2,048 cycles of products, takes some 1.9 us: the tensor pipe is busy for 52 to 62% of it, the rest is the way
 // S -> softmax (1.4 us) -> P -> S through four barriers.  Without the maximum or without the exponentials a prompt is only 6%
 // faster; two threads a row (16 softmax warps) cost 20%, S in two buffers of 64 keys 5% (an MMA of N = 64 takes as long as
-// one of N = 128), a share of the exponentials on the FMA pipes nothing.  What a call costs besides: 5 us to its first item
-// and 3 us for the join's launch, which bound the small ones; an item, 2 to 4 us of filling and draining.
+// one of N = 128), a share of the exponentials on the FMA pipes nothing.  What a call costs besides: 4 us to its first item
+// and 2 to 3 us for the join's launch, which bound the small ones; an item, 2 to 4 us of filling and draining.
 #include <limits.h>
 
 #include <atomic>
@@ -61,8 +61,9 @@ constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0,
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
 constexpr int kPaFixed2 = 260, kPaFixed1 = 120;  // cost of an item of two tiles / of one beside its keys, in keys (a step
-                                               // of 128 takes some 2 us, an item 4 or 2 us more; with 225 for both
-                                               // 192 streams took 114 us, with these 109)
+                                               // of 128 takes some 2 us, an item 4 or 2 us more; with 200 and 100
+                                               // 192 streams take 117 us, with these 101 to 109, and 6,057 tokens
+                                               // 297 against 283)
 constexpr int kPaLeast = 200;                  // least share of a block, in keys
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4;

@@ -8,6 +8,8 @@ own keys and values included (write them first); sinks fp32 [heads] or None; win
 out bf16 [tokens, heads, 128].
 
 The queries are the last tokens of their sequence: a whole prompt, a chunk behind what is cached, or drafted tokens.
+Slots of the cache that no query sees may hold anything; a value that is not finite in a slot that some queries see may
+also reach queries of the same sequence that do not.
 CUDA-graph safe: the launch depends on the shapes only; lengths and tables are read on the device.
 """
 from __future__ import annotations

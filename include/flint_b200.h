@@ -521,10 +521,9 @@ int flint_moe_grouped_down(const void* ah, const int32_t* shift, const int32_t* 
  * the tokens of b in the cache, its queries' own keys included, so query i of n sits at position p = seq_lens[b] - n + i.
  * It sees the keys max(0, p - window + 1) .. p (window 0: all up to p); a query that sees none (p < 0) gives zeros.
  * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written; out must not overlap q.  scale is
- * positive.  Slots of the cache that no
- * query sees may hold anything, NaN and infinities too; a value that is not finite in a slot that some queries see may
- * also reach queries of the same sequence that do not see it (a matrix product's 0 * NaN).  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache
- * 16-byte aligned, strides multiples of 8 elements.  workspace: flint_prefill_attention_workspace_bytes(). */
+ * positive.  Slots of the cache that no query sees may hold anything, NaN and infinities too; a value that is not finite
+ * in a slot that some queries see may also reach queries of the same sequence that do not see it (a matrix product's
+ * 0 * NaN).  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache 16-byte aligned, strides multiples of 8 elements.  workspace: flint_prefill_attention_workspace_bytes(). */
 int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads);
 int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_cache, int64_t num_blocks,
                             int64_t num_kv_heads, int64_t stride_block, int64_t stride_head, const int32_t* block_tables,
@@ -535,8 +534,10 @@ int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_ca
 /* flint_decode_attention for streams whose block tables begin with the same pages, which are read once for all of them.
  * group_starts int32 [groups + 1] (rising from 0 to batch): group g is the streams group_starts[g] ..
  * group_starts[g + 1] - 1; prefix_lens int32 [groups]: the tokens whose pages its streams share (a page that is not full
- * is not counted as shared; 0: none).  A stream's table has to name the pages up to its own length only.  seq_lens[b] counts
- * the prefix and the current token; 0 gives zeros.  Other arguments as above, q and out [batch, num_q_heads, 128]. */
+ * is not counted as shared; 0: none).  seq_lens[b] counts the prefix and the current token; 0 gives zeros.  A stream's
+ * table has to name the pages up to its own length only.  Where a window meets streams that end inside the shared prefix,
+ * the shared slots between the keys of two of them hold finite values.  Other arguments as above, q and out [batch,
+ * num_q_heads, 128]. */
 int64_t flint_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads,
                                                       int64_t num_kv_heads);
 int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, const void* kv_cache, int64_t num_blocks,
