@@ -523,7 +523,8 @@ int flint_moe_grouped_down(const void* ah, const int32_t* shift, const int32_t* 
  * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written; out must not overlap q.  scale is
  * positive.  Slots of the cache that no query sees may hold anything, NaN and infinities too; a value that is not finite
  * in a slot that some queries see may also reach queries of the same sequence that do not see it (a matrix product's
- * 0 * NaN).  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache 16-byte aligned, strides multiples of 8 elements.  workspace: flint_prefill_attention_workspace_bytes(). */
+ * 0 * NaN).  num_q_heads / num_kv_heads in 1..8; q, out and kv_cache 16-byte aligned, strides multiples of 8 elements.
+ * workspace: flint_prefill_attention_workspace_bytes(). */
 int64_t flint_prefill_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads);
 int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_cache, int64_t num_blocks,
                             int64_t num_kv_heads, int64_t stride_block, int64_t stride_head, const int32_t* block_tables,
