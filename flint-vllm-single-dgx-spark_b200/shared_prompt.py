@@ -4,6 +4,7 @@
     dec.reserve_history(n); dec.capture()
     dec.read_prompt(prompt, room=n)     # prompt attention over all its tokens; stream 0 forked into the others
     tokens = dec.decode(n)              # one CUDA graph per step; the shared pages are read once per layer and step
+                                        # (steps beyond the room, counted wherever they are run, are refused)
     dec.branch([3, 5], [0, 0])          # streams 3 and 5 go on from where stream 0 is
     dec.compact()                       # used pages to the front of the cache
 
@@ -24,6 +25,18 @@ from .prefill_attention import flint_prefill_attention
 from .shared_prefix_attention import flint_shared_prefix_attention
 
 
+class _CountedSteps:
+    """The step graph of `dec`, whose every replay takes one of the steps that read_prompt left room for."""
+
+    def __init__(self, graph, dec):
+        self.graph, self.dec = graph, dec
+
+    def replay(self):
+        self.dec._check_room(1)
+        self.dec.steps_left -= 1
+        self.graph.replay()
+
+
 class SharedPromptDecoder(Decoder):
     def __init__(self, model, streams: int, moe: str | None = None, sampling: dict | None = None):
         if model.world != 1:
@@ -36,6 +49,7 @@ class SharedPromptDecoder(Decoder):
         self.group_starts, self.prefix_lens = i32(0, streams), i32(0)
         self.all_streams = torch.arange(streams, dtype=torch.int32, device=model.dev)
         self.lens_to_come = torch.zeros_like(self.all_streams)   # tokens each stream has pages for
+        self.steps_left = None                               # steps that have pages; None: no prompt has been read
 
     # ---- decode ----
     def layer_ops(self, l):
@@ -44,6 +58,20 @@ class SharedPromptDecoder(Decoder):
             self.q.view(self.M, c.num_heads, c.head_dim), m.kv[l], self.bt, self.seq_lens, self.group_starts,
             self.prefix_lens, L["sinks"], c.window(l), self.scale, self.attn)
         return [(name, attention if name == "attention" else fn) for name, fn in super().layer_ops(l)]
+
+    def capture(self):
+        self.steps_left = None                               # (capturing writes to the first position)
+        super().capture()
+        self.graphs["step"] = _CountedSteps(self.graphs["step"], self)
+
+    def _check_room(self, n):
+        """Behind the reserved pages a step would drop its K and V and attend to keys that are not there."""
+        if n > (self.steps_left or 0):
+            raise ValueError(f"{n} steps: the room of read_prompt holds {self.steps_left or 0} more")
+
+    def decode(self, n: int):
+        self._check_room(n)
+        return super().decode(n)
 
     def _set_state(self, tokens, positions):
         dev = self.m.dev
@@ -108,8 +136,9 @@ class SharedPromptDecoder(Decoder):
         c, m, pool, dev = self.c, self.m, self.pool, self.m.dev
         ids = torch.as_tensor(np.asarray(prompt, np.int64), device=dev)
         n = ids.numel() - 1                                   # tokens whose K and V the cache takes now
-        if n < 0 or n + 1 + room > m.blocks_per_stream * PAGE:
+        if n < 0 or room < 0 or n + 1 + room > m.blocks_per_stream * PAGE:
             raise ValueError(f"a prompt of {n + 1} tokens and {room} more do not fit {m.blocks_per_stream * PAGE}")
+        self.steps_left = None
         pool.free(self.all_streams)
         if n:
             pool.reserve([0], [n])
@@ -140,10 +169,13 @@ class SharedPromptDecoder(Decoder):
         self.step_ctr.zero_()
         torch.cuda.synchronize()
         self.check_status()
+        self.steps_left = room + 1                            # the first one writes the last prompt token's K and V
 
     def branch(self, dst, src):
         """Streams dst[i] (host ints) give up their own continuation and go on from where stream src[i] is."""
         pool, dev = self.pool, self.m.dev
+        if self.steps_left is None:
+            raise ValueError("branch: no prompt yet: read_prompt() first")
         if (len(src) != len(dst) or len(set(dst)) != len(dst) or set(src) & set(dst)
                 or any(not 0 <= b < self.M for b in (*src, *dst))):
             raise ValueError(f"branch: {dst} from {src} among {self.M} streams")
