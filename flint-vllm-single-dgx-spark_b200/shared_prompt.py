@@ -82,8 +82,9 @@ class SharedPromptDecoder(Decoder):
     def _follow_tables(self):
         """seq_lens and slots from positions and the tables (a stream without a page there writes nothing)."""
         self.seq_lens.copy_(self.positions + 1)
-        page = self.bt.gather(1, (self.positions // PAGE)[:, None])[:, 0].long()
-        self.slots.copy_(torch.where(page >= 0, page * PAGE + self.positions % PAGE, -1))
+        column, width = self.positions // PAGE, self.bt.shape[1]
+        page = self.bt.gather(1, column.clamp(max=width - 1)[:, None])[:, 0].long()
+        self.slots.copy_(torch.where((page >= 0) & (column < width), page * PAGE + self.positions % PAGE, -1))
 
     def prefill(self, prompts):
         raise NotImplementedError("SharedPromptDecoder reads one prompt for all streams: read_prompt()")

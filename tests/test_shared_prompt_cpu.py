@@ -1,0 +1,28 @@
+"""SharedPromptDecoder's bookkeeping without a GPU."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+
+def decoder(streams=2, blocks=10, max_ctx=160):
+    """A decoder whose model, pool and graphs are stand-ins: only what the host decides is real."""
+    from flint_b200.shared_prompt import SharedPromptDecoder
+    dec = object.__new__(SharedPromptDecoder)
+    dec.M, dec.graphs, dec.replays = streams, {}, 0
+    dec.m = SimpleNamespace(dev="cpu", blocks_per_stream=blocks, cos_sin=torch.zeros(max_ctx, 128), embed=torch.zeros(64, 8))
+    dec.bt = torch.arange(streams * blocks, dtype=torch.int32).view(streams, blocks)
+    dec.tokens, dec.seq_lens = torch.zeros(streams, dtype=torch.int32), torch.zeros(streams, dtype=torch.int32)
+    dec.positions, dec.slots = torch.zeros(streams, dtype=torch.int64), torch.zeros(streams, dtype=torch.int64)
+    dec.history = torch.zeros((streams, 40), dtype=torch.int32)
+    return dec
+
+
+def test_positions_behind_the_table_have_no_slot(fb):
+    dec = decoder()
+    dec.bt[1, 3:] = -1
+    for at, slots in (([5, 47], [5, 207]), ([159, 48], [159, -1]), ([160, 170], [-1, -1])):
+        dec.positions.copy_(torch.tensor(at))
+        dec._follow_tables()
+        assert dec.slots.tolist() == slots and dec.seq_lens.tolist() == [at[0] + 1, at[1] + 1]
