@@ -132,13 +132,16 @@ class SharedPromptDecoder(Decoder):
     def read_prompt(self, prompt, room: int):
         """Every stream goes on from `prompt` (token ids), with pages for `room` more tokens.  Leaves the state at the
         last prompt token, as Decoder.prefill does: the first step reads it and draws each stream's first token."""
+        m, prompt = self.m, np.asarray(prompt, np.int64)
+        n = prompt.size - 1                                   # tokens whose K and V the cache takes now
+        # (the last page may reach behind the rotary table, which has a row for each position)
+        most = min(m.blocks_per_stream * PAGE, m.cos_sin.shape[0])
+        if n < 0 or room < 0 or n + 1 + room > most:
+            raise ValueError(f"a prompt of {n + 1} tokens and {room} more do not fit {most}")
         if not self.graphs:
             self.capture()
-        c, m, pool, dev = self.c, self.m, self.pool, self.m.dev
-        ids = torch.as_tensor(np.asarray(prompt, np.int64), device=dev)
-        n = ids.numel() - 1                                   # tokens whose K and V the cache takes now
-        if n < 0 or room < 0 or n + 1 + room > m.blocks_per_stream * PAGE:
-            raise ValueError(f"a prompt of {n + 1} tokens and {room} more do not fit {m.blocks_per_stream * PAGE}")
+        c, pool, dev = self.c, self.pool, m.dev
+        ids = torch.as_tensor(prompt, device=dev)
         self.steps_left = None
         pool.free(self.all_streams)
         if n:

@@ -26,3 +26,20 @@ def test_positions_behind_the_table_have_no_slot(fb):
         dec.positions.copy_(torch.tensor(at))
         dec._follow_tables()
         assert dec.slots.tolist() == slots and dec.seq_lens.tolist() == [at[0] + 1, at[1] + 1]
+
+
+class Untouchable:
+    def __getattr__(self, name):
+        raise AssertionError(f"went on to {name}")
+
+
+def test_prompts_end_with_the_rotary_table(fb):
+    """Pages are whole, so they may hold more tokens than the model has positions for."""
+    dec = decoder(blocks=10, max_ctx=150)
+    dec.c, dec.graphs, dec.pool = None, {"step": None}, Untouchable()
+    for length, room in ((145, 6), (151, 0), (1, 150)):
+        with pytest.raises(ValueError, match="do not fit 150"):
+            dec.read_prompt(np.zeros(length, np.int64), room)
+    dec.all_streams = torch.arange(2, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="went on to free"):
+        dec.read_prompt(np.zeros(145, np.int64), 5)
