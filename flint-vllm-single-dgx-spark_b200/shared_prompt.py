@@ -138,6 +138,8 @@ class SharedPromptDecoder(Decoder):
         most = min(m.blocks_per_stream * PAGE, m.cos_sin.shape[0])
         if n < 0 or room < 0 or n + 1 + room > most:
             raise ValueError(f"a prompt of {n + 1} tokens and {room} more do not fit {most}")
+        if prompt.min() < 0 or prompt.max() >= m.embed.shape[0]:
+            raise ValueError(f"token ids must lie in 0 .. {m.embed.shape[0] - 1}, got {prompt.min()} .. {prompt.max()}")
         if not self.graphs:
             self.capture()
         c, pool, dev = self.c, self.pool, m.dev

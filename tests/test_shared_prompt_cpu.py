@@ -43,3 +43,12 @@ def test_prompts_end_with_the_rotary_table(fb):
     dec.all_streams = torch.arange(2, dtype=torch.int32)
     with pytest.raises(AssertionError, match="went on to free"):
         dec.read_prompt(np.zeros(145, np.int64), 5)
+
+
+@pytest.mark.parametrize("prompt", [[1, 64, 2], [-1, 3], [3, 4, 64], [10 ** 12]])
+def test_prompt_tokens_are_in_the_vocabulary(fb, prompt):
+    dec = decoder()
+    dec.c, dec.graphs, dec.pool = None, {"step": None}, Untouchable()
+    dec.all_streams = torch.arange(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="token ids"):
+        dec.read_prompt(prompt, 3)
