@@ -34,6 +34,7 @@ class _CountedSteps:
     def replay(self):
         self.dec._check_room(1)
         self.dec.steps_left -= 1
+        self.dec.steps_done += 1
         self.graph.replay()
 
 
@@ -50,6 +51,7 @@ class SharedPromptDecoder(Decoder):
         self.all_streams = torch.arange(streams, dtype=torch.int32, device=model.dev)
         self.lens_to_come = torch.zeros_like(self.all_streams)   # tokens each stream has pages for
         self.steps_left = None                               # steps that have pages; None: no prompt has been read
+        self.steps_done = 0                                  # since the prompt was read: the column of the next tokens
 
     # ---- decode ----
     def layer_ops(self, l):
@@ -70,8 +72,13 @@ class SharedPromptDecoder(Decoder):
             raise ValueError(f"{n} steps: the room of read_prompt holds {self.steps_left or 0} more")
 
     def decode(self, n: int):
+        """n steps -> their tokens [streams, n] (int32, on the device, a view of the history)."""
         self._check_room(n)
-        return super().decode(n)
+        first = self.steps_done
+        if first + n > self.history.shape[1]:
+            raise ValueError(f"the history holds {self.history.shape[1]} steps, {first} are done: reserve_history() for all")
+        super().decode(n)
+        return self.history[:, first:first + n]
 
     def _set_state(self, tokens, positions):
         dev = self.m.dev
@@ -175,6 +182,7 @@ class SharedPromptDecoder(Decoder):
         self.step_ctr.zero_()
         torch.cuda.synchronize()
         self.check_status()
+        self.steps_done = 0
         self.steps_left = room + 1                            # the first one writes the last prompt token's K and V
 
     def branch(self, dst, src):

@@ -39,3 +39,20 @@ def test_steps_end_with_the_room(fb):
     with pytest.raises(ValueError, match="room"):
         dec.decode(1)                                             # capturing runs a step of its own: the prompt is gone
     dec.close()
+
+
+def test_decode_gives_the_tokens_of_its_own_steps(fb):
+    from flint_b200.shared_prompt import SharedPromptDecoder
+    model = build(fb)
+    dec = SharedPromptDecoder(model, 3, sampling=dict(temperature=1.0, top_k=20, top_p=1.0, seeds=[1, 2, 3]))
+    dec.reserve_history(10)
+    dec.capture()
+    prompt, runs = np.random.default_rng(6).integers(0, VOCAB, size=30), []
+    for parts in ((10,), (4, 5, 1)):
+        dec.read_prompt(prompt, room=20)
+        runs.append([dec.decode(n).cpu().numpy() for n in parts])
+        assert [t.shape for t in runs[-1]] == [(3, n) for n in parts]
+        with pytest.raises(ValueError, match="history"):
+            dec.decode(1)                                         # ten are recorded
+    np.testing.assert_array_equal(runs[0][0], np.concatenate(runs[1], axis=1))
+    dec.close()
