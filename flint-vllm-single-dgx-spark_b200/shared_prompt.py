@@ -123,17 +123,25 @@ class SharedPromptDecoder(Decoder):
         cos, sin = cos_sin[:, None].chunk(2, -1)
         return torch.cat([a * cos - b * sin, b * cos + a * sin], -1).bfloat16()
 
+    @staticmethod
+    def _router_logits(xn, gate):
+        return torch.mm(xn, gate.t(), out_dtype=torch.float32).bfloat16().float()
+
+    @staticmethod
+    def _choose(logits, ew):
+        """-> (experts, weights) [tokens, topk]: the largest logits, ties to the lower id, their scores over their sum."""
+        value, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
+        value, ids = value[:, :ew.topk], ids[:, :ew.topk].to(torch.int32).contiguous()
+        weight = torch.softmax(value, -1) if ew.score_fn == 0 else torch.sigmoid(value)
+        return ids, weight / weight.sum(-1, keepdim=True)
+
     def _experts(self, xn, L):
         T, ew = xn.shape[0], L["experts"]
         one = lambda w: grouped_moe(xn, torch.zeros((T, 1), dtype=torch.int32, device=xn.device),
                                     torch.ones((T, 1), device=xn.device), w)
         if L["gate"] is None:
             return one(ew)
-        logits = torch.mm(xn, L["gate"].t(), out_dtype=torch.float32).bfloat16().float()
-        value, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
-        value, ids = value[:, :ew.topk], ids[:, :ew.topk].to(torch.int32).contiguous()
-        weight = torch.softmax(value, -1) if ew.score_fn == 0 else torch.sigmoid(value)
-        out = grouped_moe(xn, ids, weight / weight.sum(-1, keepdim=True), ew)
+        out = grouped_moe(xn, *self._choose(self._router_logits(xn, L["gate"]), ew), ew)
         return out if ew.shared is None else out + one(ew.shared)
 
     def read_prompt(self, prompt, room: int):
