@@ -675,6 +675,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
   } else if (warp == 8) {
     // ---- TMA ----
     int slot = 0, parity = 1, nq = 0, sent = 0, q_sent = 0;       // an empty ring's slots count as released
+    int none = 0;                                                 // negative: a page that the table does not have
     bool ok = true;
     for (int n = 0; pa_all(ok); ++n) {
       if (!pa_all(pa_wait(&b_item[n % kPaQueue], (unsigned)((n / kPaQueue) & 1), &s_failed, status))) break;
@@ -693,6 +694,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         const int p0 = it.begin / kPaPage + j * 8;
         if (held != j >> 2) {
           held = j >> 2;
+          none |= ids;
           const int p = it.begin / kPaPage + held * 32 + lane;
           ids = p < pages_end ? row[p] : a.num_blocks;
         }
@@ -737,7 +739,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         else ++vj;
         if (n == 0 && i == 0 && lane == 0) FLINT_TL(5);
       }
+      none |= ids;
     }
+    if (__any_sync(0xffffffffu, none < 0) && lane == 0) atomicOr(status, STATUS_BAD_SEQ);
     if (lane == 0) s_sent[0] = sent, s_sent[1] = q_sent;
   } else if (warp == 9) {
     // ---- MMA ----

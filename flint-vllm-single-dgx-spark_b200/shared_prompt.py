@@ -62,8 +62,11 @@ class SharedPromptDecoder(Decoder):
         return [(name, attention if name == "attention" else fn) for name, fn in super().layer_ops(l)]
 
     def capture(self):
-        self.steps_left = None                               # (capturing writes to the first position)
-        super().capture()
+        self.steps_left = None
+        self.pool.free(self.all_streams)
+        self.pool.reserve(self.all_streams, torch.ones_like(self.all_streams))
+        super().capture()                                    # runs one step, at the first position
+        self.pool.free(self.all_streams)
         self.graphs["step"] = _CountedSteps(self.graphs["step"], self)
 
     def _check_room(self, n):

@@ -87,8 +87,10 @@ enum {
 enum {
   FLINT_STATUS_WAIT_TIMEOUT = 1,  /* a bounded wait gave up: that launch's outputs are invalid */
   FLINT_STATUS_BAD_EXPERT = 2,    /* a routed expert id outside 0..E-1 (clamped) */
-  FLINT_STATUS_BAD_SEQUENCE = 4,  /* a sequence longer than its block table (clamped to the table); of the page
-                                     operations: a stream, length, page or table that does not fit (left out) */
+  FLINT_STATUS_BAD_SEQUENCE = 4,  /* a sequence longer than its block table (clamped to the table; prompt and
+                                     shared-prefix attention: also one whose table has a negative entry below its
+                                     length, whose keys and values there are zeros); of the page operations: a stream,
+                                     length, page or table that does not fit (left out) */
   FLINT_STATUS_NO_PAGES = 8       /* a page operation asked for more pages than are free (that request is left out) */
 };
 /* Byte offset of the status word inside a workspace of `kind`, or -1 for an unknown kind (no GPU needed). */
@@ -537,7 +539,7 @@ int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_ca
  * group_starts[g + 1] - 1; prefix_lens int32 [groups]: the tokens whose pages its streams share (a page that is not full
  * is not counted as shared; 0: none).  seq_lens[b] counts the prefix and the current token; 0 gives zeros.  A stream's
  * table has to name the pages up to its own length only.  Where a window meets streams that end inside the shared prefix,
- * the shared slots between the keys of two of them hold finite values.  Other arguments as above, q and out [batch,
+ * the shared slots between the keys of two of them exist and hold finite values.  Other arguments as above, q and out [batch,
  * num_q_heads, 128]. */
 int64_t flint_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads,
                                                       int64_t num_kv_heads);
