@@ -6,7 +6,8 @@
 // With c = scale * log2(e), a row over its visible keys keeps a reference m, l = sum 2^(c (s - m)) and o = sum 2^(..) v in
 // 32 bits; the probabilities are rounded to bf16 for the product with V only (l sums the unrounded ones, as the decode
 // attention does).  Results over disjoint keys join as m = max m_k, l = sum l_k 2^(c (m_k - m)), o likewise.  A sink adds
-// 2^(sink log2 e - c m) to l.  A row without keys gives zeros.
+// 2^(sink log2 e - c m) to l.  A row without keys gives zeros: its l is 0.  m alone does not tell, since a maximum passes over
+// NaN: a row whose scores are NaN has m = -inf and l = NaN, and gives NaN.
 //
 // Work.  An item is one KV head and up to two row tiles of 128 rows: floor(128 / G) consecutive query tokens (or streams)
 // with their G heads each, so the group reads its keys once.  Items are laid on one line by what they cost (their keys and a
@@ -1050,10 +1051,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                w[i] = m == -INFINITY ? 0u : pa_pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                w[i] = l == 0.f ? 0u : pa_pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
               pa_store64(dst + 32 * quarter, w, a.wide);
             }
-          } else if (writes && m != -INFINITY) {
+          } else if (writes && l != 0.f) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
@@ -1100,8 +1101,9 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedAttnArgs 
   float m, l;
   float4 o;
   auto add = [&](float2 ml, float4 x) {
-    if (ml.x == -INFINITY) return;
-    const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c), f1 = pa_ex2((ml.x - mm) * a.c);
+    if (ml.y == 0.f) return;
+    const float mm = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.f : pa_ex2((m - mm) * a.c),
+                f1 = ml.x == -INFINITY ? 0.f : pa_ex2((ml.x - mm) * a.c);    // (of NaN: 0 times it stays NaN)
     l = l * f0 + ml.y * f1;
     o.x = o.x * f0 + x.x * f1, o.y = o.y * f0 + x.y * f1, o.z = o.z * f0 + x.z * f1, o.w = o.w * f0 + x.w * f1;
     m = mm;
@@ -1120,7 +1122,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedAttnArgs 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = c0 + i * Groups;
-        if (ml[i].x != -INFINITY) x[i] = __ldcg(a.o + ((2 * c + (c == first)) * 32 + quad) * 256 + row);
+        if (ml[i].y != 0.f) x[i] = __ldcg(a.o + ((2 * c + (c == first)) * 32 + quad) * 256 + row);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) add(ml[i], x[i]);
@@ -1140,7 +1142,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedAttnArgs 
     if (!valid || group != 0) return;
     float den = l;
     if (a.sinks && m != -INFINITY) den += pa_ex2(a.sinks[qh] * kPaLog2e - m * a.c);
-    const float inv = m == -INFINITY ? 0.f : 1.0f / den;
+    const float inv = l == 0.f ? 0.f : 1.0f / den;
     const uint2 w = make_uint2(pa_pack(o.x * inv, o.y * inv), pa_pack(o.z * inv, o.w * inv));
     reinterpret_cast<uint2*>(a.out + tok * a.out_stride + qh * kPaD)[quad] = w;
   };
@@ -1167,7 +1169,7 @@ __global__ void __launch_bounds__(256, 4) paged_join_kernel(const PagedAttnArgs 
     } else if (group == 0) {
       const int64_t row = (int64_t)(home * a.batch + tok) * Hq + qh;
       const float2 ml = a.home_ml[row];
-      if (ml.x != -INFINITY) add(ml, a.home_o[row * 32 + quad]);
+      if (ml.y != 0.f) add(ml, a.home_o[row * 32 + quad]);
     }
   };
   begin();

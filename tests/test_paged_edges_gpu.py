@@ -11,6 +11,58 @@ from test_paged_attention_gpu import D, PAGE, SCALE, close, make_cache, run_pref
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
 
+# ---- values that are not numbers ----
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("q_lens,lens,window", [([17], [17], 0), ([40, 3], [300, 40], 0), ([2], [9000], 0), ([150], [400], 37),
+                                                ([20], [12], 0)])
+def test_prefill_query_that_is_not_a_number(fb, q_lens, lens, window, sinks):
+    """A row of q with a NaN gives NaN where it sees keys (zeros where it sees none); no other row changes a bit."""
+    from flint_b200 import prefill_attention as pa
+    args, out = run_prefill(np.random.default_rng(31 + len(lens)), q_lens, lens, 2, 4, window, sinks)
+    want = host(out).copy()
+    for row, head in ((0, 3), (1, 0), (q_lens[0] - 1, 7)):
+        args[0][row, head, 5] = float("nan")
+        if lens[0] - q_lens[0] + row >= 0:
+            want[row, head] = np.nan
+    out.zero_()
+    pa.flint_prefill_attention(*args)
+    np.testing.assert_array_equal(host(out), want)
+
+
+@pytest.mark.parametrize("first,last", [(4096, 4097), (4000, 5000), (0, 9000), (8999, 9000), (100, 8900)])
+def test_prefill_keys_that_are_not_numbers(fb, first, last):
+    """Keys of NaN in a long cache reach every row that sees one of them, wherever the line of items is cut."""
+    from flint_b200 import prefill_attention as pa
+    n, rows = 9000, 3
+    args, out = run_prefill(np.random.default_rng(33), [rows, 5], [n, 40], 2, 8, 0, True)
+    want, bt = host(out).copy(), args[2].cpu()
+    for j in range(first, last):
+        args[1][int(bt[0, j // PAGE]), 1, j % PAGE, 7] = float("nan")
+    want[[i for i in range(rows) if n - rows + i >= first], 8:] = np.nan
+    out.zero_()
+    pa.flint_prefill_attention(*args)
+    np.testing.assert_array_equal(host(out), want)
+
+
+@pytest.mark.parametrize("first,last", [(0, 1024), (300, 301), (1030, 1090)])
+def test_shared_keys_and_queries_that_are_not_numbers(fb, first, last):
+    from flint_b200 import shared_prefix_attention as sp
+    lens = [1030, 1100, 0, 1025, 1200, 1024]
+    args, out = run_shared(np.random.default_rng(34), [6], [1024], lens, 2, 8, 0, True)
+    want, bt = host(out).copy(), args[2].cpu()
+    for j in range(first, last):
+        args[1][int(bt[4, j // PAGE]), 0, j % PAGE, 100] = float("nan")
+    args[0][:3, 11, 0] = float("nan")
+    for b, n in enumerate(lens):
+        if n > first and (first < 1024 or b == 4):                # (stream 4's own keys are its alone)
+            want[b, :8] = np.nan
+        if b < 3 and n:
+            want[b, 11] = np.nan
+    out.zero_()
+    sp.flint_shared_prefix_attention(*args)
+    np.testing.assert_array_equal(host(out), want)
+
+
 # ---- tables that end before their streams do ----
 def test_missing_pages_are_reported(fb):
     """A page below a row's length whose table entry is negative is a sequence longer than its table; entries that no row
