@@ -830,14 +830,19 @@ def _(q, kv_cache, block_tables, seq_lens, sinks, window, scale, out, splits):
 # ------------------------------------------------------------------------------------------------------------
 # prompts and shared prompts over the paged cache
 # ------------------------------------------------------------------------------------------------------------
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, int, float, type(None)))
+
+
 def run(name: str, *args) -> None:
     """Op `name` of this section.  Its Python function is called directly, since the dispatcher's way to a Python kernel
-    takes more host time (20 of 40 us a call) than these launches; through torch.ops where a tracer or a dispatch mode
-    has to see the op."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
-        getattr(torch.ops.flint_b200, name)(*args)
-    else:
-        _DIRECT[name](*args)
+    takes more host time (20 of 40 us a call) than these launches; through torch.ops where a tracer, a dispatch mode or a
+    tensor's subclass has to see the op.  The tensors that it writes count a version either way."""
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or not _PLAIN.issuperset(map(type, args))):
+        return getattr(torch.ops.flint_b200, name)(*args)
+    fn, written = _DIRECT[name]
+    fn(*args)
+    torch._C._increment_version([args[i] for i in written])
 
 
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
@@ -1067,8 +1072,10 @@ def _(kv, ref, block_tables, num_pages, remap, live):
     return None
 
 
-_DIRECT = dict(prefill_attention=_prefill_attention, shared_prefix_attention=_shared_prefix_attention,
-               kv_reserve=_kv_reserve, kv_fork=_kv_fork, kv_free=_kv_free, kv_compact=_kv_compact)
+# the functions, and the places of the arguments that they write (the ops' mutates_args)
+_DIRECT = dict(prefill_attention=(_prefill_attention, (8,)), shared_prefix_attention=(_shared_prefix_attention, (9,)),
+               kv_reserve=(_kv_reserve, (0, 1, 2)), kv_fork=(_kv_fork, (0, 1, 2, 3, 4)), kv_free=(_kv_free, (0, 1, 2, 3)),
+               kv_compact=(_kv_compact, (0, 1, 2, 4, 5)))
 
 
 # ------------------------------------------------------------------------------------------------------------

@@ -90,3 +90,31 @@ def test_missing_pages_are_reported(fb):
             with report():
                 fb._lib.check_device_status()
         fb._lib.check_device_status()
+
+
+# ---- what autograd is told ----
+def test_calls_are_seen_by_autograd(fb):
+    """Written tensors count a version, as through the registered ops."""
+    from flint_b200 import kv_pages
+    from flint_b200 import prefill_attention as pa
+    from flint_b200 import shared_prefix_attention as sp
+    args, out = run_prefill(np.random.default_rng(51), [5], [30], 2, 4, 0, False)
+    was = out._version
+    pa.flint_prefill_attention(*args)
+    assert out._version > was
+    saved = torch.ones_like(out, requires_grad=True)
+    product = (saved * out).sum()                                 # keeps out for its backward pass
+    pa.flint_prefill_attention(*args)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    args, out = run_shared(np.random.default_rng(52), [2], [32], [40, 50], 2, 4, 0, False)
+    was = out._version
+    sp.flint_shared_prefix_attention(*args)
+    assert out._version > was
+    pool = kv_pages.PagePool(torch.zeros((1, 9, 1, PAGE, 256), dtype=torch.bfloat16, device="cuda"), 3, 4)
+    versions = lambda: [t._version for t in (pool.kv, *pool.state, pool.remap, pool.live)]
+    for call, written in ((lambda: pool.reserve([0], [40]), [0, 1, 1, 0, 1, 0, 0]), (lambda: pool.fork([0], [1]), [1, 1, 1, 1, 1, 0, 0]),
+                          (lambda: pool.free([0]), [0, 1, 1, 1, 1, 0, 0]), (lambda: pool.compact(), [1, 1, 1, 0, 0, 1, 1])):
+        was = versions()
+        call()
+        assert [int(b > a) for a, b in zip(was, versions())] == written
