@@ -32,7 +32,7 @@ struct KvPagesWorkspace {
   int moves;                                     // compact: pages to move
   unsigned pad[30];
 };
-// behind it the plan: fork -- int4 (from row, to row, whole pages, tail page taken from) and int (tail page) per request;
+// behind it the plan: fork -- int4 (from row, to row, tokens, started page taken from) and int (its copy) per request;
 // compact -- int2 (from, to) per move
 
 struct KvPool {
@@ -187,26 +187,31 @@ __global__ void __launch_bounds__(kPgT) kv_reserve_kernel(const KvPool p, const 
   pg_publish();
 }
 
-// One block.  Checks the forks, takes a page for each tail, writes the children's counts and the plan of the copies.
+// One block.  Checks the forks, takes a page for each tail and writes the plan of the copies.  (The ids of the source's full
+// pages are checked by the block that copies them, which is what makes the child: here they would cost a walk of every row.)
 __global__ void __launch_bounds__(kPgT) kv_fork_plan_kernel(const KvPool p, const int* src, const int* dst, int n) {
   __shared__ int red[32], fresh[kPgMaxRequests];
   extern __shared__ int claim[];
   pdl_trigger();                                                  // the copying launch may line up
   pdl_wait();
   pg_claim(dst, n, p.streams, claim);
-  int len[kPgPer], mine = 0;                                      // len < 0: no fork
+  int len[kPgPer], last[kPgPer], mine = 0;                        // len < 0: no fork; last: its source's started page
   bool tail[kPgPer];
 #pragma unroll
   for (int j = 0; j < kPgPer; ++j) {
     const int i = threadIdx.x * kPgPer + j;
-    len[j] = -1, tail[j] = false;
+    len[j] = last[j] = -1, tail[j] = false;
     if (i >= n) continue;
     const int s = src[i], d = dst[i];
     bool ok = s >= 0 && s < p.streams && d >= 0 && d < p.streams && s != d && claim[d] == i && p.num_pages[d] == 0;
     if (ok) {
       const int L = p.seq_lens[s], pages = L / kPgPage + (L % kPgPage != 0);
       ok = L >= 0 && pages <= p.num_pages[s] && pages <= p.max_blocks;
-      if (ok) len[j] = L, tail[j] = L % kPgPage != 0;
+      if (ok && L % kPgPage != 0) {
+        last[j] = p.tables[(int64_t)s * p.bt_stride + L / kPgPage];
+        ok = tail[j] = last[j] >= 0 && last[j] < p.blocks;
+      }
+      if (ok) len[j] = L;
     }
     if (!ok) atomicOr(&p.ws->status, STATUS_BAD_STREAM);
     mine += tail[j];
@@ -230,21 +235,14 @@ __global__ void __launch_bounds__(kPgT) kv_fork_plan_kernel(const KvPool p, cons
     int4 plan = make_int4(-1, -1, 0, -1);
     int to = -1;
     if (len[j] >= 0) {
-      const int whole = len[j] / kPgPage;
       bool ok = true;
       if (tail[j]) {
-        const int page = p.tables[(int64_t)src[i] * p.bt_stride + whole];
         ok = at < limit;
         if (!ok) atomicOr(&p.ws->status, STATUS_NO_PAGES);
         else to = fresh[at];
         ++at;
-        plan.w = page;
       }
-      if (ok) {
-        plan = make_int4(src[i], dst[i], whole, plan.w);
-        p.num_pages[dst[i]] = whole + tail[j];
-        p.seq_lens[dst[i]] = len[j];
-      }
+      if (ok) plan = make_int4(src[i], dst[i], len[j], last[j]);
     }
     pg_fork_plan(p)[i] = plan;
     pg_fork_tail(p)[i] = to;
@@ -256,7 +254,8 @@ __device__ __forceinline__ void pg_copy(uint4* dst, const uint4* src, int units)
   for (int u = threadIdx.x; u < units; u += blockDim.x) dst[u] = src[u];
 }
 
-// grid (1 + layers, requests): the first block of a request writes its table row, the others copy its tail page.
+// grid (1 + layers, requests): the first block of a request makes the child, the others copy its source's started page (of no
+// use, and to a page that is free again, where a full page's id is bad).
 __global__ void __launch_bounds__(256) kv_fork_kernel(const KvPool p, uint4* kv, int64_t layer_units, int64_t block_units,
                                                       int units) {
   pdl_wait();
@@ -266,21 +265,29 @@ __global__ void __launch_bounds__(256) kv_fork_kernel(const KvPool p, uint4* kv,
   if (blockIdx.x == 0) {
     const int* from = p.tables + (int64_t)f.x * p.bt_stride;
     int* row = p.tables + (int64_t)f.y * p.bt_stride;
-    for (int i = threadIdx.x; i < f.z; i += 256) {
-      const int page = from[i];
-      row[i] = page;
-      if (page >= 0 && page < p.blocks) atomicAdd(&p.ref[page], 1);
-      else atomicOr(&p.ws->status, STATUS_BAD_STREAM);
+    const int whole = f.z / kPgPage;
+    bool bad = false;
+    for (int i = threadIdx.x; i < whole; i += 256) bad |= (unsigned)from[i] >= (unsigned)p.blocks;
+    if (__syncthreads_or(bad)) {                                  // left out whole; its page goes back
+      if (threadIdx.x == 0) {
+        atomicOr(&p.ws->status, STATUS_BAD_STREAM);
+        if (to >= 0) atomicSub(&p.ref[to], 1);
+      }
+    } else {
+      for (int i = threadIdx.x; i < whole; i += 256) {
+        row[i] = from[i];
+        atomicAdd(&p.ref[from[i]], 1);
+      }
+      if (threadIdx.x == 0) {
+        if (to >= 0) row[whole] = to;
+        p.num_pages[f.y] = whole + (to >= 0);
+        p.seq_lens[f.y] = f.z;
+      }
     }
-    if (to >= 0 && threadIdx.x == 0) row[f.z] = to;
     pg_publish();
     return;
   }
   if (to < 0) return;
-  if (f.w < 0 || f.w >= p.blocks) {
-    if (threadIdx.x == 0) atomicOr(&p.ws->status, STATUS_BAD_STREAM);
-    return;
-  }
   uint4* layer = kv + (blockIdx.x - 1) * layer_units;
   pg_copy(layer + to * block_units, layer + f.w * block_units, units);
   pg_publish();

@@ -118,3 +118,31 @@ def test_calls_are_seen_by_autograd(fb):
         was = versions()
         call()
         assert [int(b > a) for a, b in zip(was, versions())] == written
+
+
+# ---- page operations on tables that do not fit ----
+@pytest.mark.parametrize("column,entry", [(0, -1), (1, 99), (2, -7), (2, 40)])
+def test_fork_of_a_bad_table_is_left_out_whole(fb, column, entry):
+    """An id outside the pool among the source's full pages (0, 1) or as its started page (2): no child, no page taken, the
+    other forks of the call as ever."""
+    from flint_b200 import kv_pages
+    fb._lib.device_status(clear=True)
+    kv = torch.randn((2, 40, 1, PAGE, 256), device="cuda").bfloat16()
+    pool = kv_pages.PagePool(kv, 6, 9)
+    pool.reserve([2, 4], [45, 20])
+    pool.seq_lens.copy_(torch.tensor([0, 0, 45, 0, 20, 0], dtype=torch.int32))
+    pool.block_tables[2, column] = entry
+    before = [t.clone() for t in pool.state]
+    pool.fork([2, 4, 2], [0, 3, 5])
+    with pytest.raises(fb._lib.FlintError, match="did not fit"):
+        fb._lib.check_device_status()
+    ref, tables, lens, num = (t.clone() for t in pool.state)
+    for s in (0, 5):
+        assert num[s] == 0 and lens[s] == 0 and (tables[s] == -1).all()
+    child = int(tables[3, 1])
+    assert num[3] == 2 and lens[3] == 20 and tables[3, 0] == before[1][4, 0] and torch.equal(kv[:, child], kv[:, int(tables[4, 1])])
+    want = before[0].clone()
+    want[int(tables[4, 0])] += 1
+    want[child] += 1
+    assert torch.equal(ref, want) and (before[0][child] == 0)
+    assert all(torch.equal(a[[1, 2, 4]], b[[1, 2, 4]]) for a, b in zip((tables, lens, num), before[1:]))
