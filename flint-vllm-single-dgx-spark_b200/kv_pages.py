@@ -4,14 +4,16 @@ The cache of all layers is one bf16 tensor ``kv`` [layers, blocks, kv_heads, 16,
 the device: ``ref`` [blocks] (how many streams hold a page, 0: free), ``block_tables`` [streams, max_blocks] (-1 behind a
 stream's pages), ``seq_lens`` and ``num_pages`` [streams].  Every call runs on the current stream without reading anything
 back; pages come from the lowest free ids in the order of the call's streams, so equal states give equal results.  A
-request that does not fit is left out whole and recorded in the device status (``_lib.check_device_status``).
+request that does not fit is left out whole and recorded in the device status (``_lib.check_device_status``); behind the
+first that finds too few free pages, every later one of the call that needs a page is refused too.
 
 * ``flint_kv_reserve(ref, block_tables, seq_lens, num_pages, streams, lens)`` -- room for lens[i] tokens in streams[i]
+  (seq_lens is there so that the pool's state can be passed as one; it is neither read nor written)
 * ``flint_kv_fork(kv, ref, block_tables, seq_lens, num_pages, src, dst)`` -- the empty stream dst[i] becomes a copy of
   src[i]: whole pages shared, the last page copied in every layer if it is not full
-* ``flint_kv_free(ref, block_tables, seq_lens, num_pages, streams)``
+* ``flint_kv_free(ref, block_tables, seq_lens, num_pages, streams)`` -- a stream named twice is freed once
 * ``flint_kv_compact(kv, ref, block_tables, num_pages, remap, live)`` -- used pages to the ids 0 .. live - 1;
-  remap int32 [blocks] tells where a used page went (-1: free), live int32 [1] their number
+  remap int32 [blocks] tells where a used page went (-1: free), live int32 [1] their number (num_pages is not read)
 
 ``PagePool`` keeps the tensors of one cache together.
 """

@@ -557,14 +557,20 @@ int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, const void*
  * (0: free); block_tables int32 [num_streams, max_blocks], -1 behind a stream's pages; num_pages and seq_lens int32
  * [num_streams].  An empty pool is all zeros with tables of -1.  Pages are taken from the lowest free ids in the order
  * of the call's streams, so the same state gives the same pages.  streams / src / dst / lens are device int32 [n], n and
- * num_streams up to 4,096.  A request that does not fit (an id out of range, a stream named twice: the first stands; a
- * length behind the table; too few free pages) is left out whole and recorded in the status word.
+ * num_streams up to 4,096.  A request that does not fit (an id out of range; in reserve and fork
+ * a stream named twice: the first stands; a length behind the table; too few free pages) is left out whole and recorded
+ * in the status word.  Free pages are counted in the call's order and a refused request keeps its place: behind the first
+ * that finds too few, every later one that needs a page finds too few as well.
  *   flint_kv_reserve: stream streams[i] gets pages until it has room for lens[i] tokens (never fewer than it has)
  *   flint_kv_fork:    empty stream dst[i] (num_pages 0) becomes a copy of src[i]: full pages shared, the last page, if
- *                     not full, copied in every layer into a page of its own; pages reserved ahead are not inherited
- *   flint_kv_free:    streams give their pages back
+ *                     not full, copied in every layer into a page of its own; pages reserved ahead are not inherited.
+ *                     A source whose table names a page outside the pool is left out (if that is a full page, the page
+ *                     taken for the copy is free again only after the call)
+ *   flint_kv_free:    streams give their pages back; an empty stream, or one named twice, has none to give and is not
+ *                     recorded; an entry outside the pool, or of a page that is free already, is recorded and dropped
  *   flint_kv_compact: the used pages behind the first `live` (their number) move, in rising order, to the free ids among
  *                     the first `live`; tables follow.  remap int32 [blocks]: where a used page is now, -1: free
+ *                     (num_pages is checked as the pool's, not read)
  * workspace: flint_kv_pages_workspace_bytes(blocks), one for all four. */
 int64_t flint_kv_pages_workspace_bytes(int64_t blocks);
 int flint_kv_reserve(int32_t* ref, int64_t blocks, int32_t* block_tables, int64_t bt_stride, int64_t max_blocks,

@@ -146,3 +146,16 @@ def test_fork_of_a_bad_table_is_left_out_whole(fb, column, entry):
     want[child] += 1
     assert torch.equal(ref, want) and (before[0][child] == 0)
     assert all(torch.equal(a[[1, 2, 4]], b[[1, 2, 4]]) for a, b in zip((tables, lens, num), before[1:]))
+
+
+def test_refusals_keep_their_place_and_repeats_are_freed_once(fb):
+    from flint_b200 import kv_pages
+    fb._lib.device_status(clear=True)
+    pool = kv_pages.PagePool(torch.zeros((1, 6, 1, PAGE, 256), dtype=torch.bfloat16, device="cuda"), 5, 4)
+    pool.reserve([0, 1, 2, 3, 4], [40, 64, 16, 0, 10])            # 3 of 6; 4 of 3: refused, and so are 2 and 4
+    assert pool.num_pages.tolist() == [3, 0, 0, 0, 0] and pool.ref.tolist() == [1, 1, 1, 0, 0, 0]
+    with pytest.raises(fb._lib.FlintError, match="fewer pages were free"):
+        fb._lib.check_device_status()
+    pool.free([0, 0, 3])
+    assert pool.num_pages.tolist() == [0] * 5 and pool.ref.tolist() == [0] * 6
+    fb._lib.check_device_status()
