@@ -887,9 +887,16 @@ def _check_int32(what, name, t, n, dev):
 
 
 @functools.lru_cache(maxsize=256)
-def _bytes_of(fn: str, *sizes) -> int:
-    """A workspace's size: a function of the sizes alone."""
+def _bytes_of(dev: int, fn: str, *sizes) -> int:
+    """A workspace's size: a function of the sizes and of the device's multiprocessors (dev is the current device)."""
     return int(getattr(lib(), fn)(*sizes))
+
+
+def _workspace(what, dev: int, kind: str, *sizes) -> tuple[int, int]:
+    """-> (workspace, stream).  The library launches on the current device, with as many blocks as that one takes."""
+    if dev != torch._C._cuda_getDevice():
+        raise _lib.FlintError(f"{what}: tensors on cuda:{dev}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+    return _lib.workspace_and_stream(dev, kind, _bytes_of(dev, f"flint_{kind}_workspace_bytes", *sizes))
 
 
 def _prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -903,8 +910,7 @@ def _prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: to
     if T == 0 or B == 0:
         return
     L = lib()
-    ws, stream = _lib.workspace_and_stream(dev, "prefill_attention",
-                                           _bytes_of("flint_prefill_attention_workspace_bytes", B, T, Hq, args[4]))
+    ws, stream = _workspace("prefill_attention", dev, "prefill_attention", B, T, Hq, args[4])
     rc = L.flint_prefill_attention(*args, cu_seqlens.data_ptr(), seq_lens.data_ptr(), ptr(sinks), window, scale, B, T, Hq,
                                    out.data_ptr(), out_stride, ws, PDL, stream)
     if rc:
@@ -934,8 +940,7 @@ def _shared_prefix_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     if B == 0:
         return
     L = lib()
-    ws, stream = _lib.workspace_and_stream(dev, what, _bytes_of("flint_shared_prefix_attention_workspace_bytes", B, n, Hq,
-                                                                args[4]))
+    ws, stream = _workspace(what, dev, what, B, n, Hq, args[4])
     rc = L.flint_shared_prefix_attention(*args, seq_lens.data_ptr(), group_starts.data_ptr(), prefix_lens.data_ptr(), n,
                                          ptr(sinks), window, scale, B, Hq, out.data_ptr(), out_stride, ws, PDL, stream)
     if rc:
@@ -980,9 +985,8 @@ def _check_kv(what, kv, ref):
     return (kv.data_ptr(), shape[0], shape[2], st[0] if shape[0] > 1 else page * shape[1], st[1] if shape[1] > 1 else page)
 
 
-def _pages_ws(ref):
-    ws, stream = _lib.workspace_and_stream(ref.get_device(), "kv_pages",
-                                           _bytes_of("flint_kv_pages_workspace_bytes", ref.numel()))
+def _pages_ws(what, ref):
+    ws, stream = _workspace(what, ref.get_device(), "kv_pages", ref.numel())
     return ws, PDL, stream
 
 
@@ -994,7 +998,7 @@ def _kv_reserve(ref: torch.Tensor, block_tables: torch.Tensor, num_pages: torch.
     _check_int32("kv_reserve", "lens", lens, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_reserve(*pool, streams.data_ptr(), lens.data_ptr(), n, *_pages_ws(ref))
+    rc = L.flint_kv_reserve(*pool, streams.data_ptr(), lens.data_ptr(), n, *_pages_ws("kv_reserve", ref))
     if rc:
         check(rc, "flint_kv_reserve")
 
@@ -1016,7 +1020,7 @@ def _kv_fork(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor, se
     _check_int32("kv_fork", "dst", dst, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_fork(*cache, *pool, src.data_ptr(), dst.data_ptr(), n, *_pages_ws(ref))
+    rc = L.flint_kv_fork(*cache, *pool, src.data_ptr(), dst.data_ptr(), n, *_pages_ws("kv_fork", ref))
     if rc:
         check(rc, "flint_kv_fork")
 
@@ -1037,7 +1041,7 @@ def _kv_free(ref: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tens
     _check_int32("kv_free", "streams", streams, n, ref.get_device())
     if n == 0:
         return
-    rc = L.flint_kv_free(*pool, streams.data_ptr(), n, *_pages_ws(ref))
+    rc = L.flint_kv_free(*pool, streams.data_ptr(), n, *_pages_ws("kv_free", ref))
     if rc:
         check(rc, "flint_kv_free")
 
@@ -1058,7 +1062,7 @@ def _kv_compact(kv: torch.Tensor, ref: torch.Tensor, block_tables: torch.Tensor,
     cache = _check_kv("kv_compact", kv, ref)
     _check_int32("kv_compact", "remap", remap, ref.numel(), ref.get_device())
     _check_int32("kv_compact", "live", live, 1, ref.get_device())
-    rc = L.flint_kv_compact(*cache, *pool, remap.data_ptr(), live.data_ptr(), *_pages_ws(ref))
+    rc = L.flint_kv_compact(*cache, *pool, remap.data_ptr(), live.data_ptr(), *_pages_ws("kv_compact", ref))
     if rc:
         check(rc, "flint_kv_compact")
 

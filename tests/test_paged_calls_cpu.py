@@ -33,3 +33,24 @@ def test_subclasses_see_the_registered_op(fb):
     assert seen == ["flint_b200.kv_free"]
     with pytest.raises(fb._lib.FlintError, match="CUDA"):
         kv_pages.flint_kv_free(i(9), i(2, 3), i(2), torch.nn.Parameter(i(2), requires_grad=False), i(1))
+
+
+def test_workspaces_are_sized_for_their_device(fb, monkeypatch):
+    """A size found on one device is not another's, and a call for another device than the current one is refused: the
+    launch takes the current device's number of blocks."""
+    ops, current, sized = fb.ops, [0], []
+
+    class Library:
+        def flint_kv_pages_workspace_bytes(self, blocks):
+            return blocks * (100 + current[0])
+
+    monkeypatch.setattr(ops, "lib", Library)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(fb._lib, "workspace_and_stream", lambda dev, kind, n: sized.append((dev, kind, n)) or (1, 2))
+    blocks = 7919
+    for current[0] in (0, 1):
+        assert ops._workspace("kv_free", current[0], "kv_pages", blocks) == (1, 2)
+    assert sized == [(0, "kv_pages", 100 * blocks), (1, "kv_pages", 101 * blocks)]
+    with pytest.raises(fb._lib.FlintError, match="cuda:0, but the current device is cuda:1"):
+        ops._workspace("kv_free", 0, "kv_pages", blocks)
+    ops._bytes_of.cache_clear()
