@@ -159,3 +159,83 @@ def test_refusals_keep_their_place_and_repeats_are_freed_once(fb):
     pool.free([0, 0, 3])
     assert pool.num_pages.tolist() == [0] * 5 and pool.ref.tolist() == [0] * 6
     fb._lib.check_device_status()
+
+
+# ---- many sequences, long prompts, head groups ----
+@pytest.mark.parametrize("batch", [1100, 2100])
+def test_prefill_many_sequences(fb, batch):
+    """More sequences than are kept in shared memory while the items are cut (2,048), and more than one lane-full of runs."""
+    rng = np.random.default_rng(batch)
+    q_lens = [int(x) for x in rng.integers(0, 4, size=batch)]
+    run_prefill(rng, q_lens, [n + int(x) for n, x in zip(q_lens, rng.integers(0, 50, size=batch))], 1, 2, 0, True)
+
+
+@pytest.mark.parametrize("groups", [600, 1100])
+def test_shared_many_groups(fb, groups):
+    rng = np.random.default_rng(groups)
+    sizes = [1 if i % 7 else 2 for i in range(groups)]
+    prefix = [int(x) * PAGE for x in rng.integers(0, 4, size=groups)]
+    lens = [p + int(x) for p, n in zip(prefix, sizes) for x in rng.integers(0, 40, size=n)]
+    run_shared(rng, sizes, prefix, lens, 1, 2, 0, False)
+
+
+@pytest.mark.parametrize("n,past,Hkv,G,window", [(4100, 0, 4, 8, 0), (5003, 0, 1, 3, 0), (2050, 6001, 2, 8, 0),
+                                                 (4500, 333, 2, 4, 700)])
+def test_prefill_long_prompts(fb, n, past, Hkv, G, window):
+    """Prompts of many items to a block, compared at the rows beside every item's ends and at random ones."""
+    from flint_b200 import prefill_attention as pa
+    rng = np.random.default_rng(n)
+    tables = scattered(rng, [-(-(n + past) // PAGE)])
+    kv, bt = make_cache(rng, tables, [n + past], Hkv)
+    q = bf16(rng, (n, Hkv * G, D), 2.0)
+    out = torch.empty((n, Hkv * G, D), dtype=torch.bfloat16, device="cuda")
+    pa.flint_prefill_attention(dev_bf16(q), dev_bf16(kv), to_dev(bt), to_dev(np.array([0, n], np.int32)),
+                               to_dev(np.array([n + past], np.int32)), None, window or None, SCALE, out)
+    got, tile = host(out), 2 * (128 // G)
+    assert np.isfinite(got).all()
+    rows = sorted({0, n - 1, *rng.integers(0, n, size=40).tolist(),
+                   *[r for i in rng.integers(1, n // tile, size=15).tolist() for r in (i * tile - 1, i * tile)]})
+    k, v = paged.cached(kv, bt[0], n + past)
+    for r in rows:
+        want, spread = paged.attention_rows(q[r:r + 1], k, v, past + r, None, window, SCALE)
+        close(got[r:r + 1], want, spread, f"row {r} of {n}")
+
+
+@pytest.mark.parametrize("Hkv", [1, 3])
+def test_six_heads_to_a_group(fb, Hkv):
+    run_prefill(np.random.default_rng(61), [3, 0, 64, 1, 33], [43, 5, 64, 1, 233], Hkv, 6, 0, True)
+    run_shared(np.random.default_rng(62), [2, 1, 4], [64, 0, 320], [70, 81, 9, 321, 322, 400, 336], Hkv, 6, 0, True)
+
+
+# ---- calls that follow one another without a pause ----
+def test_attention_right_behind_page_operations(fb):
+    """The decode attention looks at lengths, tables and older pages before its wait on the call before it: what it reads
+    right behind a fork, a compaction or a reservation is what it reads after a pause."""
+    from flint_b200 import decode_attention as da
+    from flint_b200 import kv_pages
+    rng = np.random.default_rng(71)
+    kv = torch.randn((24, 700, 4, PAGE, 2 * D), device="cuda").bfloat16()
+    q = dev_bf16(bf16(rng, (1, 32, D))).expand(8, -1, -1).contiguous()
+    n = 1003
+    for turn in range(12):
+        pool = kv_pages.PagePool(kv, 8, 80)
+        pool.reserve([6, 3], [160, n])                            # a stream in front, so that compaction moves pages
+        pool.seq_lens[3] = n
+        others = torch.tensor([0, 1, 2, 4, 5, 7], dtype=torch.int32, device="cuda")
+        source, gone = torch.full_like(others, 3), torch.tensor([6], dtype=torch.int32, device="cuda")
+        outs = [torch.empty_like(q) for _ in range(3)]
+        torch.cuda.synchronize()
+        pool.fork(source, others)
+        da.flint_decode_attention(q, kv[turn], pool.block_tables, pool.seq_lens, None, None, SCALE, outs[0])
+        pool.free(gone)
+        da.flint_decode_attention(q, kv[turn], pool.block_tables, pool.seq_lens, None, None, SCALE, outs[1])
+        pool.compact()
+        da.flint_decode_attention(q, kv[turn], pool.block_tables, pool.seq_lens, None, None, SCALE, outs[2])
+        after = torch.empty_like(q)
+        torch.cuda.synchronize()
+        da.flint_decode_attention(q, kv[turn], pool.block_tables, pool.seq_lens, None, None, SCALE, after)
+        others = others.long().tolist()
+        for o in outs + [after]:
+            for b in (3, *others):
+                np.testing.assert_array_equal(host(o[b]), host(after[3]), err_msg=f"turn {turn}, stream {b}")
+            assert (host(o[6]) == 0).all()
