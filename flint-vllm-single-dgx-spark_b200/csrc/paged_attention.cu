@@ -1264,10 +1264,13 @@ static int paged_attn(const void* q, int64_t q_stride, const void* kv, int64_t n
   // A prompt's item is cut between its steps, and tables of eight pages hold one step (17 tokens: 10.9 us on the device
   // without the join, 12.9 with it).
   if (!group_starts && max_blocks * kPaPage <= kPaKeys) return FLINT_OK;
-  // Few rows are cut into many parts, which four groups share (8 streams on a 6,048-token prefix, 256 rows in some 30 parts:
-  // 28 us a call against 31); many rows keep the SMs full by themselves (6,057 tokens: 294 us against 347).
+  // Four groups share a row's parts where one pass of blocks then takes all rows, since each pass costs a chain of loads.
+  // Streams: their blocks of two rows are resident at once (four an SM).  32 heads on 4 KV heads and a 6,048-token prefix, four
+  // groups / one: 256 rows 22.7 / 26.2 us a call, 1,024 rows 26.7 / 28.2, 2,048 rows 35.0 / 32.4, 4,096 rows 53 / 45.
+  // Prompts: an item's eight blocks of two rows hold all that a KV head has.  Behind 6,057 tokens, 8 rows 19.4 / 22.5 us,
+  // 32 rows 25.6 / 23.0, 64 rows 37.7 / 24.2.
   const int64_t rows = (group_starts ? batch : tokens) * Hq;
-  const int per_block = rows <= (group_starts ? 4096 : 256) ? 2 : 8;
+  const int per_block = (group_starts ? rows <= 2 * 4 * blocks : tokens * G <= 2 * kPaJoin) ? 2 : 8;
   const dim3 grid((unsigned)(group_starts ? (rows + per_block - 1) / per_block : (int64_t)blocks * kPaJoin));
   return per_block == 2 ? launch(paged_join_kernel<4>, grid, dim3(256), 0, stream, pdl, a, blocks)
                         : launch(paged_join_kernel<1>, grid, dim3(256), 0, stream, pdl, a, blocks);
