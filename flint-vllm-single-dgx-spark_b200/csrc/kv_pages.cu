@@ -12,8 +12,9 @@
 // a page of a layer (8 KB a KV head) to a block at a time.
 //
 // Measured: 386 pages of a pool of 1,536 moved in 48 layers (1.21 GB read and written) 219 us, 5.5 TB/s or 85% of the copy
-// rate; free, fork of 40 of 64 streams on a 6,057-token prompt with their last pages in 48 layers, and reserve 26 us together
-// on the device (the pages' floor is 19 us).  A small call takes 3 to 5 us a launch on the device and 8 to 12 us of host time.
+// rate.  40 of 64 streams on a 6,057-token prompt freed and forked anew in 48 layers, 27 of them with a started page, and pages
+// reserved for all: free 3.5, fork 17.1, reserve 5.8 us on the device (27 pages written and 5 read take 7.7).  A small call takes
+// 2 to 4 us a launch on the device and 8 to 13 us of host time.
 #include "common.cuh"
 #include "runtime.cuh"
 #include "tma.cuh"

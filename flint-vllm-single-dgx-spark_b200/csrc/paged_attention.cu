@@ -27,12 +27,12 @@
 // last page, if cut, is read with its first row shifted up, so that the rows behind the end are out of bounds too, and rows
 // of V that a window has left behind in the first page are cleared in shared memory.
 //
-// Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 283 us (1.06 PFLOP/s), of 16,421 tokens 1.8 ms (1.2), in long
-// runs at the card's power limit 325 us and 2.11 ms; 192 streams on three prefixes of up to 16,384 tokens 101 us.  A step of
-// two tiles, 2,048 cycles of products, takes some 1.9 us: the tensor pipe is busy for 52 to 62% of it, the rest is the way
+// Measured (32 heads on 4 KV heads): a prompt of 6,057 tokens 284 us (1.06 PFLOP/s), of 16,421 tokens 1.9 ms (1.16), in long
+// runs at the card's power limit 327 us and 2.12 ms; 192 streams on three prefixes of up to 16,384 tokens 102 us.  A step of
+// two tiles, 2,048 cycles of products, takes some 1.9 us: the tensor pipe is busy for 51 to 62% of it, the rest is the way
 // S -> softmax (1.4 us) -> P -> S through four barriers.  Without the maximum or without the exponentials a prompt is only 6%
 // faster; two threads a row (16 softmax warps) cost 20%, S in two buffers of 64 keys 5% (an MMA of N = 64 takes as long as
-// one of N = 128), a share of the exponentials on the FMA pipes nothing.  What a call costs besides: 4 us to its first item
+// one of N = 128), a share of the exponentials on the FMA pipes nothing.  What a call costs besides: 3 to 6 us to its first item
 // and 2 to 3 us for the join's launch, which bound the small ones; an item, 2 to 4 us of filling and draining.
 #include <limits.h>
 
@@ -61,11 +61,13 @@ constexpr int kPaThreads = 384;                // 2 x 4 softmax warps, TMA, MMA,
 constexpr int kPaTmem = 512;                   // columns: S0 (P0), S1 (P1), O0, O1, 128 each
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaRise = 8.f;                 // log2 of how far p may exceed 1 before the reference moves
-constexpr int kPaFixed2 = 260, kPaFixed1 = 120;  // cost of an item of two tiles / of one beside its keys, in keys (a step
-                                               // of 128 takes some 2 us, an item 4 or 2 us more; with 200 and 100
-                                               // 192 streams take 117 us, with these 101 to 109, and 6,057 tokens
-                                               // 297 against 283)
-constexpr int kPaLeast = 200;                  // least share of a block, in keys
+// Cost of an item of two tiles / of one beside its keys, in keys (a step of 128 takes some 2 us, an item 4 or 2 us more).
+// At 130/60, 200/100, 260/120, 320/160, 400/200: 6,057 tokens 327, 298, 288, 303, 313 us; 192 streams 115, 104, 102, 106, 107;
+// packed prompts under a window 76, 74, 67, 64, 64; 1,000 tokens 38, 35, 35, 34, 37; 2,048 behind 6,057 221 to 224.
+constexpr int kPaFixed2 = 260, kPaFixed1 = 120;
+// Least share of a block, in keys.  At 100, 200, 400, 800: 17 tokens 10.8, 10.6, 14.6, 23.1 us; a row on 1,000 keys 13.9, 15.9,
+// 18.9, 26.7; four rows on 3,000 keys 22.0, 20.5, 21.8, 26.8; 2 streams 17.6, 20.1, 20.4, 28.7; 8 streams 24.0, 24.0, 24.5, 28.4.
+constexpr int kPaLeast = 200;
 constexpr unsigned STATUS_BAD_SEQ = 4u;
 constexpr size_t kPaSmem = 1024 + 2 * kPaSlotBytes + (size_t)kPaSlots * kPaSlotBytes + kPaM * 32 * 4;
 

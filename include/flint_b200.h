@@ -521,7 +521,8 @@ int flint_moe_grouped_down(const void* ah, const int32_t* shift, const int32_t* 
  * heads contiguous); kv_cache, block_tables and sinks as for flint_decode_attention.  cu_seqlens int32 [batch + 1]: the
  * query tokens of sequence b are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (none: b is skipped); seq_lens int32 [batch]:
  * the tokens of b in the cache, its queries' own keys included, so query i of n sits at position p = seq_lens[b] - n + i.
- * It sees the keys max(0, p - window + 1) .. p (window 0: all up to p); a query that sees none (p < 0) gives zeros.
+ * It sees the keys max(0, p - window + 1) .. p (window 0: all up to p); a query that sees none (p < 0) gives zeros, one
+ * whose visible scores hold a NaN gives NaN.
  * Rows of out [tokens, num_q_heads, 128] (bf16) behind cu_seqlens[batch] are not written; out must not overlap q.  scale is
  * positive.  Slots of the cache that no query sees may hold anything, NaN and infinities too; a value that is not finite
  * in a slot that some queries see may also reach queries of the same sequence that do not see it (a matrix product's
