@@ -690,6 +690,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
       if (steps == 0) continue;
       const int* row = a.block_tables + (int64_t)it.table * a.bt_stride;
       const int pages_end = (it.end + kPaPage - 1) / kPaPage;
+      // (of a prefix under a window, pages between two streams' keys may be gone by right: no row sees them)
+      const int heed = it.home && a.window > 0 ? 0 : -1;
       // table entries of four steps, one per lane; the first ones are on their way while Q is sent for
       int held = it.j0 >> 2, ids = it.begin / kPaPage + held * 32 + lane;
       ids = ids < pages_end ? row[ids] : a.num_blocks;
@@ -697,7 +699,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         const int p0 = it.begin / kPaPage + j * 8;
         if (held != j >> 2) {
           held = j >> 2;
-          none |= ids;
+          none |= ids & heed;
           const int p = it.begin / kPaPage + held * 32 + lane;
           ids = p < pages_end ? row[p] : a.num_blocks;
         }
@@ -742,7 +744,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant_
         else ++vj;
         if (n == 0 && i == 0 && lane == 0) FLINT_TL(5);
       }
-      none |= ids;
+      none |= ids & heed;
     }
     if (__any_sync(0xffffffffu, none < 0) && lane == 0) atomicOr(status, STATUS_BAD_SEQ);
     if (lane == 0) s_sent[0] = sent, s_sent[1] = q_sent;

@@ -540,8 +540,8 @@ int flint_prefill_attention(const void* q, int64_t q_stride_t, const void* kv_ca
  * group_starts[g + 1] - 1; prefix_lens int32 [groups]: the tokens whose pages its streams share (a page that is not full
  * is not counted as shared; 0: none).  seq_lens[b] counts the prefix and the current token; 0 gives zeros.  A stream's
  * table has to name the pages up to its own length only.  Where a window meets streams that end inside the shared prefix,
- * the shared slots between the keys of two of them exist and hold finite values.  Other arguments as above, q and out [batch,
- * num_q_heads, 128]. */
+ * the shared slots between the keys of two of them hold finite values (a page that the table no longer names reads as
+ * zeros, and is not reported there).  Other arguments as above, q and out [batch, num_q_heads, 128]. */
 int64_t flint_shared_prefix_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads,
                                                       int64_t num_kv_heads);
 int flint_shared_prefix_attention(const void* q, int64_t q_stride_b, const void* kv_cache, int64_t num_blocks,

@@ -92,6 +92,20 @@ def test_missing_pages_are_reported(fb):
         fb._lib.check_device_status()
 
 
+def test_pages_between_windows_may_be_gone(fb):
+    """Streams that end inside a shared prefix under a window: the shared pages between their keys are seen by no row, and a
+    table that has given them away is no fault."""
+    from flint_b200 import shared_prefix_attention as sp
+    fb._lib.check_device_status()
+    for lens, gone in (([300, 1000, 990], range(19, 32)), ([100, 500, 490], range(7, 26))):
+        args, out = run_shared(np.random.default_rng(43), [3], [512], lens, 2, 4, 64, True)
+        was = host(out).copy()
+        args[2][:, list(gone)] = -1
+        sp.flint_shared_prefix_attention(*args)
+        np.testing.assert_array_equal(host(out), was)
+        fb._lib.check_device_status()
+
+
 # ---- what autograd is told ----
 def test_calls_are_seen_by_autograd(fb):
     """Written tensors count a version, as through the registered ops."""
